@@ -67,6 +67,22 @@ class TensorRef(ctypes.Structure):
                 ("rows", ctypes.c_int64), ("cols", ctypes.c_int64)]
 
 
+class KvCache(ctypes.Structure):
+    """Mirror of ``ctb_kv_cache``."""
+
+    _fields_ = [(n, ctypes.c_void_p) for n in ("k", "v", "k_scale", "v_scale")] + [
+        (n, ctypes.c_int64) for n in ("num_blocks", "k_block_stride", "k_head_stride", "k_token_stride",
+                                      "v_block_stride", "v_head_stride", "v_token_stride")] + [
+        (n, ctypes.c_int32) for n in ("heads", "block_size", "head_dim", "dtype")]
+
+
+class KvBatch(ctypes.Structure):
+    """Mirror of ``ctb_kv_batch``."""
+
+    _fields_ = [(n, ctypes.c_void_p) for n in ("block_table", "seq_lens", "query_start")] + [
+        (n, ctypes.c_int64) for n in ("table_width", "table_stride", "tokens")] + [(n, ctypes.c_int32) for n in ("batch", "reserved")]
+
+
 _lib = None
 
 
@@ -84,6 +100,12 @@ def lib() -> ctypes.CDLL:
         _lib.ctb_launch_count.restype = ctypes.c_int64
         _lib.ctb_minmax_workspace_bytes.restype = ctypes.c_int64
         _lib.ctb_minmax_workspace_bytes.argtypes = [ctypes.c_int64] * 4
+        vp, c64, c32 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32  # declared types: plain Python numbers go through as they are
+        _lib.ctb_dequantize_linear.argtypes = [vp, vp, c64, vp, vp, vp, vp, vp, vp, vp]
+        _lib.ctb_kv_cache_append.argtypes = [vp, vp, vp, vp, c32, c64, c64, c64, c64, vp]
+        _lib.ctb_kv_cache_attention_workspace_bytes.restype = c64
+        _lib.ctb_kv_cache_attention_workspace_bytes.argtypes = [vp, vp, c32]
+        _lib.ctb_kv_cache_attention.argtypes = [vp, vp, vp, c32, c64, c64, c32, ctypes.c_float, c32, vp, vp, vp, vp]
     return _lib
 
 

@@ -17,7 +17,8 @@ __all__ = [
     "sparse24_mask", "sparse24_compress", "quantize_fp8_sparse24", "sparse24_decompress", "sparse24_decompress_dequantize_fp8", "bitmask_compress", "bitmask_decompress", "hadamard",
     "absmax_quantize", "rotate_quantize_int4_batch", "rotate_quantize_int4_batch_bounded", "quantize_pack_int4_batch",
     "unpack_dequantize_int4_batch", "quantize_fp8_channel_batch", "dequantize_fp8_channel_batch",
-    "quantize_fp4_g16_batch", "dequantize_fp4_g16_batch", "tensor_table", "QINT", "QFLOAT",
+    "quantize_fp4_g16_batch", "dequantize_fp4_g16_batch", "tensor_table", "dequantize_linear", "kv_cache_append", "kv_cache_attention",
+    "QINT", "QFLOAT",
 ]
 
 _CODEC = {"dtype": CODE_DTYPE, "pack32": CODE_PACK32, "fp4x2": CODE_FP4X2}
@@ -574,3 +575,177 @@ def unpack_dequantize_int4_batch(table, device=None):
     (words in, bf16 weights out), as one launch."""
     stream = ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
     check(lib().ctb_unpack_dequantize_int4_batch(table, i32(len(table)), stream))
+
+
+# ---------------------------------------------------------------- serving a compressed model
+
+_HALF = (torch.bfloat16, torch.float16)
+
+
+def _same_device(first, *rest):
+    require_cuda(first, *rest)
+    for t in rest:
+        if t is not None and t.device != first.device:
+            raise ValueError(f"all tensors of a call must be on one device, got {first.device} and {t.device}")
+
+
+def _call(device, fn, *args):
+    """`fn(*args, stream)` with `device` current, on its current stream."""
+    stream = torch.cuda.current_stream(device).cuda_stream
+    if device.index == torch.cuda.current_device():
+        check(fn(*args, stream))
+    else:
+        with torch.cuda.device(device):
+            check(fn(*args, stream))
+
+
+def _dp(t):
+    return None if t is None else t.data_ptr()
+
+
+def dequantize_linear(x, q, scale, zp=None, *, qtype, bits=4, col_group, scale_row_stride, codec="pack32", global_scale=None, bias=None):
+    """x @ dequantize(q, scale, zp).T + bias without the dense weight in memory, for few tokens (every 32 read `q` again).
+
+    x [..., cols] bf16 / f16; q as `dequantize` takes it: int32 words [rows, ceil(cols / 8)] (codec "pack32", qtype QINT) or
+    uint8 pairs [rows, cols / 2] (codec "fp4x2", qtype QFLOAT); scale, zp (int8) and global_scale as there; bias [rows] of
+    x's dtype.  The dequantized weight is not rounded: products and sums are fp32, the result is rounded once."""
+    if codec not in ("pack32", "fp4x2"):
+        raise NotImplementedError(f"the product takes packed codes (pack32, fp4x2), got {codec!r}")
+    if bits != 4 or qtype != (QINT if codec == "pack32" else QFLOAT):
+        raise NotImplementedError("the product is built for 4-bit codes: int in pack32, float in fp4x2")
+    if x.dtype not in _HALF:
+        raise TypeError(f"x must be bfloat16 or float16, got {x.dtype}")
+    if q.dtype is not (torch.int32 if codec == "pack32" else torch.uint8) or q.dim() != 2:
+        raise TypeError(f"q must be a 2-D {'int32' if codec == 'pack32' else 'uint8'} tensor of packed codes, got {q.dim()}-D {q.dtype}")
+    if x.dim() < 1:
+        raise ValueError("x needs a column dimension")
+    rows, cols = q.shape[0], x.shape[-1]
+    if q.shape[1] != ((cols + 7) // 8 if codec == "pack32" else cols // 2) or (codec == "fp4x2" and cols % 2):
+        raise ValueError(f"packed weight of shape {tuple(q.shape)} does not hold {cols} columns")
+    if scale.dtype not in (*_HALF, torch.float32, torch.float8_e4m3fn):
+        raise TypeError(f"unsupported scale dtype {scale.dtype}")
+    if rows and cols:
+        if col_group < 1 or cols % col_group:
+            raise ValueError(f"tensor column shape must be divisble by the given group_size {col_group} but got {cols}")
+        if scale_row_stride < 0:
+            raise ValueError("scale_row_stride must not be negative")
+        need = (rows - 1) * scale_row_stride + cols // col_group
+        for name, t in (("scale", scale), ("zp", zp)):
+            if t is not None and t.numel() < need:
+                raise ValueError(f"{name} holds {t.numel()} entries, {need} are read")
+    if zp is not None:
+        if codec == "fp4x2":
+            raise NotImplementedError("fp4 codes have no zero point")
+        if zp.dtype is not torch.int8:
+            raise TypeError(f"zp must be int8, got {zp.dtype}")
+    if global_scale is not None:
+        if codec != "fp4x2":
+            raise NotImplementedError("a global scale belongs to fp4 codes")
+        if global_scale.numel() != 1:
+            raise ValueError("global_scale holds one value")
+    if bias is not None and (bias.dtype is not x.dtype or tuple(bias.shape) != (rows,)):
+        raise ValueError(f"bias must be a {x.dtype} tensor of shape ({rows},)")
+    _same_device(x, q, scale, zp, bias)
+    x, q, scale, zp, bias = _c(x), _c(q), _c(scale), _c(zp), _c(bias)
+    out = torch.empty(x.shape[:-1] + (rows,), dtype=x.dtype, device=x.device)
+    d = QDesc(rows, cols, col_group, 1, scale_row_stride, qtype, bits, DT[x.dtype], DT[scale.dtype], L.I8, 0, _CODEC[codec], 0)
+    gs = _gs(global_scale, x)
+    tokens = x.numel() // cols if cols else out.numel() // max(rows, 1)
+    _call(x.device, lib().ctb_dequantize_linear, ctypes.addressof(d), x.data_ptr(), tokens, q.data_ptr(), scale.data_ptr(), _dp(zp),
+          _dp(gs), _dp(bias), out.data_ptr())
+    return out
+
+
+def _rows_of_heads(t, name, heads, dim):
+    """[tokens, heads, dim] with contiguous heads and 16-byte steps: as it is where it has them (a slice of a fused
+    projection does), else a copy."""
+    if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != dim:
+        raise ValueError(f"{name} must be [tokens, {heads}, {dim}], got {tuple(t.shape)}")
+    if dim > 1 and t.stride(2) != 1:
+        return t.contiguous()
+    return t
+
+
+def _kv_structs(x, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, query_start):
+    """Checks what append and attention share and builds their descriptors; returns them with what has to stay alive."""
+    if k_cache.dim() != 4 or v_cache.shape != k_cache.shape:
+        raise ValueError(f"k_cache and v_cache must be [num_blocks, heads, block_size, head_dim], got {tuple(k_cache.shape)} and {tuple(v_cache.shape)}")
+    if k_cache.dtype not in (torch.int8, torch.float8_e4m3fn) or v_cache.dtype is not k_cache.dtype:
+        raise TypeError(f"the cache holds int8 or float8_e4m3fn codes, got {k_cache.dtype} and {v_cache.dtype}")
+    if x.dtype not in _HALF:
+        raise TypeError(f"queries, keys and values must be bfloat16 or float16, got {x.dtype}")
+    blocks, heads, size, dim = k_cache.shape
+    if heads < 1 or size < 1:
+        raise ValueError("the cache needs at least one head and one slot per block")
+    if not 1 <= dim <= 256:
+        raise NotImplementedError(f"head sizes up to 256 are built, got {dim}")
+    for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
+        if t.stride(3) != 1 and dim > 1:
+            raise ValueError(f"{name}: the last dimension must be contiguous")
+    for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
+        if t.dtype is not torch.float32 or tuple(t.shape) != (blocks, heads) or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous float32 tensor of shape ({blocks}, {heads})")
+    for name, t, n in (("block_table", block_table, 2), ("seq_lens", seq_lens, 1), ("query_start", query_start, 1)):
+        if t.dtype not in (torch.int32, torch.int64) or t.dim() != n:
+            raise TypeError(f"{name} must be a {n}-D int32 or int64 tensor")
+    batch = seq_lens.shape[0]
+    if block_table.shape[0] != batch or query_start.shape[0] != batch + 1:
+        raise ValueError(f"{batch} lengths need a block table of {batch} rows and {batch + 1} row offsets, got {block_table.shape[0]} and {query_start.shape[0]}")
+    _same_device(x, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, query_start)
+    block_table, seq_lens, query_start = (t if t.dtype is torch.int32 else t.to(torch.int32) for t in (block_table, seq_lens, query_start))
+    if block_table.stride(1) != 1 and block_table.shape[1] > 1:
+        block_table = block_table.contiguous()
+    seq_lens, query_start = seq_lens.contiguous(), query_start.contiguous()
+    ks, vs = k_cache.stride(), v_cache.stride()
+    c = L.KvCache(k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), blocks, ks[0], ks[1], ks[2],
+                  vs[0], vs[1], vs[2], heads, size, dim, DT[k_cache.dtype])
+    b = L.KvBatch(block_table.data_ptr(), seq_lens.data_ptr(), query_start.data_ptr(), block_table.shape[1], block_table.stride(0),
+                  x.shape[0], batch, 0)
+    return c, b, (block_table, seq_lens, query_start)
+
+
+def kv_cache_append(k, v, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, query_start) -> None:
+    """Quantizes the rows k, v [tokens, heads, head_dim] (bf16 / f16) into an 8-bit paged cache, in place.
+
+    k_cache, v_cache [num_blocks, heads, block_size, head_dim] int8 or float8_e4m3fn (any strides, head_dim contiguous);
+    k_scale, v_scale float32 [num_blocks, heads]; block_table [batch, width]; seq_lens [batch]: tokens of each request,
+    these rows included; query_start [batch + 1]: row offsets.  Row i of request b goes to position
+    seq_lens[b] - (query_start[b + 1] - query_start[b]) + i, slot position % block_size of block
+    block_table[b, position // block_size].  The scale of a (block, head) is the symmetric min-max scale of the rows
+    written to it; where the block already holds tokens of the request it never shrinks, and when it grows the older codes are
+    rounded again.  Positions outside the table and blocks outside the cache are left out.  A block that is written must
+    belong to one request."""
+    if k_cache.dim() == 4:
+        k, v = (_rows_of_heads(t, n, k_cache.shape[1], k_cache.shape[3]) for t, n in ((k, "k"), (v, "v")))
+    if k.dtype is not v.dtype or k.shape != v.shape:
+        raise ValueError(f"k and v must have one shape and dtype, got {tuple(k.shape)} {k.dtype} and {tuple(v.shape)} {v.dtype}")
+    c, b, keep = _kv_structs(k, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, query_start)
+    _same_device(k, v)
+    _call(k.device, lib().ctb_kv_cache_append, ctypes.addressof(c), ctypes.addressof(b), k.data_ptr(), v.data_ptr(), DT[k.dtype],
+          k.stride(0), k.stride(1), v.stride(0), v.stride(1))
+
+
+def kv_cache_attention(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, query_start, softmax_scale=None, causal=True,
+                       return_lse=False):
+    """softmax(q k^T * softmax_scale) v over an 8-bit paged cache (laid out as for kv_cache_append) -> [tokens, q_heads, head_dim].
+
+    q [tokens, q_heads, head_dim] bf16 / f16, q_heads a multiple of the cache's heads (query head h reads cache head
+    h // (q_heads // heads)); rows query_start[b] .. query_start[b + 1] are the last tokens of request b, whose keys and
+    values are in the cache already.  softmax_scale defaults to head_dim ** -0.5.  With `causal` a query sees the positions
+    up to its own, otherwise all of its request.  Queries that see nothing give zeros.  return_lse: also the logarithm of the
+    softmax denominator, float32 [tokens, q_heads] (-inf for those queries)."""
+    if k_cache.dim() == 4:
+        heads, dim = k_cache.shape[1], k_cache.shape[3]
+        if q.dim() != 3 or q.shape[2] != dim or q.shape[1] < 1 or q.shape[1] % max(heads, 1):
+            raise ValueError(f"q must be [tokens, a multiple of {heads}, {dim}], got {tuple(q.shape)}")
+        q = _rows_of_heads(q, "q", q.shape[1], dim)
+    c, b, keep = _kv_structs(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, query_start)
+    tokens, q_heads, dim = q.shape
+    out = torch.empty((tokens, q_heads, dim), dtype=q.dtype, device=q.device)
+    lse = torch.empty((tokens, q_heads), dtype=torch.float32, device=q.device)
+    pc, pb = ctypes.addressof(c), ctypes.addressof(b)
+    nbytes = lib().ctb_kv_cache_attention_workspace_bytes(pc, pb, q_heads)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+    _call(q.device, lib().ctb_kv_cache_attention, pc, pb, q.data_ptr(), DT[q.dtype], q.stride(0), q.stride(1), q_heads,
+          dim ** -0.5 if softmax_scale is None else float(softmax_scale), int(bool(causal)), out.data_ptr(), lse.data_ptr(), _dp(ws))
+    return (out, lse) if return_lse else out

@@ -8,7 +8,8 @@ operators; the host mirror of the reference interface calls these.
 
 Operators: quantize, dequantize, fake_quantize, absmax_quantize, minmax, calculate_qparams, generate_gparam,
 pack_int32, unpack_int32, pack_fp4, unpack_fp4, pack_bitmasks, unpack_bitmasks, sparse24_mask, sparse24_compress,
-quantize_fp8_sparse24, sparse24_decompress, sparse24_decompress_dequantize_fp8, bitmask_compress, bitmask_decompress, hadamard.
+quantize_fp8_sparse24, sparse24_decompress, sparse24_decompress_dequantize_fp8, bitmask_compress, bitmask_decompress, hadamard;
+and those that serve a compressed model: dequantize_linear, kv_cache_append, kv_cache_attention.
 """
 from typing import List, Optional, Sequence, Tuple
 
@@ -403,3 +404,77 @@ OPERATORS: Sequence[str] = ("quantize", "dequantize", "fake_quantize", "absmax_q
                             "generate_gparam", "pack_int32", "unpack_int32", "pack_fp4", "unpack_fp4", "pack_bitmasks",
                             "unpack_bitmasks", "sparse24_mask", "sparse24_compress", "quantize_fp8_sparse24", "sparse24_decompress", "sparse24_decompress_dequantize_fp8",
                             "bitmask_compress", "bitmask_decompress", "hadamard")
+
+
+# ---------------------------------------------------------------- serving a compressed model
+# A decoding step makes several of these calls for a few microseconds of GPU work each, so they are registered without
+# the Python layers that custom_op puts around a call.  They compute no gradients and refuse inputs that want one.
+
+_SERVING = torch.library.Library(NS, "FRAGMENT")
+
+
+def _no_grad_wanted(name, *tensors):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError(f"{name} computes no gradients: call it under torch.no_grad(), or use the dequantized weight")
+
+
+def _define(name: str, schema: str, fn, fake) -> None:
+    _SERVING.define(f"{name}{schema}")
+    _SERVING.impl(name, fn, "CompositeExplicitAutograd")
+    torch.library.register_fake(f"{NS}::{name}", fake, lib=_SERVING)
+
+
+def _dequantize_linear(x, q, scale, zp, qtype, bits, col_group, scale_row_stride, codec, global_scale, bias):
+    return _o.dequantize_linear(x, q, scale, zp, qtype=qtype, bits=bits, col_group=col_group, scale_row_stride=scale_row_stride,
+                                codec=codec, global_scale=global_scale, bias=bias)
+
+
+def _dequantize_linear_fake(x, q, scale, zp, qtype, bits, col_group, scale_row_stride, codec, global_scale, bias):
+    return x.new_empty(tuple(x.shape[:-1]) + (q.shape[0],))
+
+
+_define("dequantize_linear", "(Tensor x, Tensor q, Tensor scale, Tensor? zp, int qtype, int bits, int col_group, int scale_row_stride, "
+        "str codec, Tensor? global_scale, Tensor? bias) -> Tensor", _dequantize_linear, _dequantize_linear_fake)
+
+
+def dequantize_linear(x, q, scale, zp=None, *, qtype, bits=4, col_group, scale_row_stride, codec="pack32", global_scale=None, bias=None):
+    _no_grad_wanted("dequantize_linear", x, q, scale, global_scale, bias)
+    return torch.ops.ctb200.dequantize_linear(x, q, scale, zp, qtype, bits, col_group, scale_row_stride, codec, global_scale, bias)
+
+
+def _kv_cache_append_fake(k, v, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, query_start):
+    return None
+
+
+_define("kv_cache_append", "(Tensor k, Tensor v, Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor(c!) k_scale, Tensor(d!) v_scale, "
+        "Tensor block_table, Tensor seq_lens, Tensor query_start) -> ()", _o.kv_cache_append, _kv_cache_append_fake)
+
+
+def kv_cache_append(k, v, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, query_start) -> None:
+    _no_grad_wanted("kv_cache_append", k, v)
+    torch.ops.ctb200.kv_cache_append(k, v, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, query_start)
+
+
+def _kv_cache_attention(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, query_start, softmax_scale, causal):
+    return _o.kv_cache_attention(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, query_start, softmax_scale, causal,
+                                 return_lse=True)
+
+
+def _kv_cache_attention_fake(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, query_start, softmax_scale, causal):
+    return q.new_empty(q.shape), q.new_empty(q.shape[:2], dtype=torch.float32)
+
+
+_define("kv_cache_attention", "(Tensor q, Tensor k_cache, Tensor v_cache, Tensor k_scale, Tensor v_scale, Tensor block_table, "
+        "Tensor seq_lens, Tensor query_start, float? softmax_scale, bool causal) -> (Tensor, Tensor)",
+        _kv_cache_attention, _kv_cache_attention_fake)
+
+
+def kv_cache_attention(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, query_start, softmax_scale=None, causal=True,
+                       return_lse=False):
+    _no_grad_wanted("kv_cache_attention", q)
+    out, lse = torch.ops.ctb200.kv_cache_attention(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, query_start,
+                                                   softmax_scale, causal)
+    return (out, lse) if return_lse else out
+
+
+SERVING_OPERATORS: Sequence[str] = ("dequantize_linear", "kv_cache_append", "kv_cache_attention")

@@ -348,6 +348,66 @@ int ctb_quantize_fp4_g16_batch(const ctb_tensor_ref *tensors, int32_t count, con
 int ctb_dequantize_fp4_g16_batch(const ctb_tensor_ref *tensors, int32_t count, const void *const *global_scales,
                                  void *stream);
 
+/* ---- serving a compressed model ---------------------------------------------------------------------------
+ * The reference stops at the checkpoint: its linear/compressed_linear.py:88-106 decompresses the whole weight before
+ * the first product, and quantization/quant_config.py kv_cache_scheme only describes a cache.  These entry points
+ * compute with the compressed forms themselves.
+ *
+ * out[t][n] = sum_k x[t][k] * w[n][k] (+ bias[n]),  w = (code - zero_point) * scale' as in ctb_dequantize, without
+ * rounding w: products and sums are held in fp32, the result is rounded once to desc->x_dtype.
+ * desc describes the weight [rows = n, cols = k]: codec PACK32 (qtype int, num_bits 4; zero_point int8 per qparam or
+ * NULL) or FP4X2 (qtype float, num_bits 4, no zero point; global_scale fp32 [1] or NULL); row_group 1; x_dtype
+ * (bf16 / f16) is the type of x [tokens, k], bias [n] (or NULL) and out [tokens, n]; all contiguous.
+ * Meant for few tokens: every 32 tokens read the weight again. */
+int ctb_dequantize_linear(const ctb_qdesc *desc, const void *x, int64_t tokens, const void *q, const void *scale,
+                          const void *zero_point, const float *global_scale, const void *bias, void *out, void *stream);
+
+/* A paged 8-bit cache: pages ("blocks") of block_size tokens, codes I8 or E4M3 addressed with element strides (the
+ * head_dim codes of a token are contiguous), one fp32 scale per (block, head): k_scale[block * heads + head]. */
+typedef struct ctb_kv_cache {
+    void *k, *v;
+    float *k_scale, *v_scale; /* [num_blocks, heads] */
+    int64_t num_blocks;
+    int64_t k_block_stride, k_head_stride, k_token_stride;
+    int64_t v_block_stride, v_head_stride, v_token_stride;
+    int32_t heads, block_size, head_dim, dtype;
+} ctb_kv_cache;
+
+/* Which tokens belong to which request.  Request b owns rows query_start[b] .. query_start[b + 1] of the token-major
+ * inputs; they are its last tokens, at positions seq_lens[b] - (number of its rows) .. seq_lens[b] - 1.  Position p
+ * lives in slot p % block_size of block block_table[b * table_stride + p / block_size].  All int32, on the device.
+ * Positions below zero or beyond table_width * block_size, and blocks outside [0, num_blocks), are left out: nothing
+ * is written to them and no query sees them. */
+typedef struct ctb_kv_batch {
+    const int32_t *block_table; /* [batch, table_width], rows table_stride apart */
+    const int32_t *seq_lens;    /* [batch]: tokens in the cache, those of this call included */
+    const int32_t *query_start; /* [batch + 1], not decreasing */
+    int64_t table_width, table_stride;
+    int64_t tokens;             /* rows of the token-major inputs */
+    int32_t batch, reserved;
+} ctb_kv_batch;
+
+/* Quantizes the rows k, v [tokens, heads, head_dim] (dtype bf16 / f16, element strides, head_dim contiguous) into the
+ * cache.  Scale of a (block, head): max(absmax / half the code range, 2^-23) as ctb_calculate_qparams has it for a
+ * symmetric type (448 for E4M3, 127.5 for I8), over the rows written by this call; where the request's block already
+ * holds tokens, the larger of that and the old scale, and if it grew, the older codes of the request are rounded
+ * again on the new scale.  Codes are the nearest grid values of the exact quotients (ties to even).  A block that is
+ * written must belong to one request only.  Rows behind query_start[batch] are ignored. */
+int ctb_kv_cache_append(const ctb_kv_cache *cache, const ctb_kv_batch *batch, const void *k, const void *v, int32_t dtype,
+                        int64_t k_token_stride, int64_t k_head_stride, int64_t v_token_stride, int64_t v_head_stride,
+                        void *stream);
+
+/* out [tokens, q_heads, head_dim] (q's dtype, contiguous) = softmax(softmax_scale * q k^T) v over the request's cached
+ * tokens; query head h reads cache head h / (q_heads / heads).  With `causal` a query sees positions up to its own,
+ * otherwise all seq_lens[b].  lse [tokens, q_heads] fp32 = log of the softmax denominator (natural, maximum included).
+ * Queries that see nothing (empty requests, rows behind query_start[batch]) give zeros and an lse of -infinity.
+ * q [tokens, q_heads, head_dim]: bf16 / f16, element strides, head_dim contiguous; head_dim <= 256.
+ * workspace: ctb_kv_cache_attention_workspace_bytes() bytes of device scratch, contents ignored. */
+int64_t ctb_kv_cache_attention_workspace_bytes(const ctb_kv_cache *cache, const ctb_kv_batch *batch, int32_t q_heads);
+int ctb_kv_cache_attention(const ctb_kv_cache *cache, const ctb_kv_batch *batch, const void *q, int32_t dtype,
+                           int64_t q_token_stride, int64_t q_head_stride, int32_t q_heads, float softmax_scale,
+                           int32_t causal, void *out, float *lse, void *workspace, void *stream);
+
 /* ---- staging memory of the host <-> device pipeline ------------------------------------------------------
  * The reference keeps a state dict in ordinary host memory and never leaves the CPU
  * (compressors/quantized_compressors/base.py:74, :125 compression_device="cpu").  Here host-resident tensors are
