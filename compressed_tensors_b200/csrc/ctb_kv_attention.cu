@@ -1,0 +1,714 @@
+// Attention over the 8-bit paged cache for few query rows per cache head (decoding): head sizes 64, 128 and 256, blocks of
+// a multiple of 16 tokens.
+//
+// What bounds it: every cached byte is read once per row tile and used for a handful of query rows, so the call takes the
+// time of reading the cache from HBM.
+//
+// A step is 16 cached tokens of one head, which lie in one block: one key scale, one value scale.  With query rows as
+// the 8 columns of mma.m16n8k16,
+//     S^T [16 tokens, 8 rows] = K [16, D] Q^T,      O^T [D, 8 rows] += V^T [D, 16] P^T,
+// both products take the cache as the 16-row operand, so the codes go from 16-byte loads into operand registers without a
+// transpose through shared memory: the order of the contracted index is free (d in the first product, tokens in the second),
+// and so is the order of the rows of O^T.  Only P^T changes layout (movmatrix, one 8 x 8 tile each).
+//
+// Number formats.  Codes become f16 exactly (e4m3 and int8 both fit).  A query row is scaled by a power of two to a
+// largest element in [128, 256) and held in f16: bf16 elements are exact down to 2^-24 of the largest one.  Weights are f16 as
+// well: P' = 2^(s + log2 v_scale - m), where m follows the maximum of s + log2 v_scale (of what a token weighs with its
+// scale), so the tokens that matter have f16's 11 bits whatever the scales of their blocks are; the denominator is the fp32
+// sum of P' / v_scale before that rounding.  Scores, m, sums and O are fp32.
+//
+// m is raised only where a score passes it by more than 2^8, which f16 has room for: in nearly every step the decision is
+// one vote, and nothing is exchanged between lanes or rescaled.
+//
+// Work.  The steps of all (request, row tile, head) items form one line that is cut into equal pieces, one per
+// block, whatever the lengths are; a piece's parts of an item that other pieces share go to scratch as (O, m, sum), and the
+// second kernel joins them.  The warps of a block take every fourth step and join in shared memory.  Each warp keeps
+// kAttStages steps in flight with cp.async: a lane copies the pieces that it will itself read, so its own wait is enough.
+#include <atomic>
+
+#include "ctb_fastdiv.h"
+#include "ctb_kv_common.cuh"
+#include "ctb_mma.cuh"
+
+namespace ctb {
+
+constexpr int kAttWarps = 4, kAttThreads = kAttWarps * 32, kAttMinPiece = 16;
+
+// What the second kernel has to know of the item that begins in a piece and ends behind it: written by the piece's block.
+struct AttJoin {
+    int64_t row;               // row of out and lse of the item's first query row's head 0 within the cache head
+    int64_t slot;              // of the first part; the others follow at slots 2p (p on a padded line), p = piece + 1 .. last
+    uint32_t last;             // last piece; 0: there is no such item
+    int32_t rows, first;       // query rows of the tile; which of the cache head's query heads the first one is
+    int32_t padded;
+};
+
+struct AttArgs {
+    ctb_kv_cache c;
+    ctb_kv_batch t;
+    const void *q;
+    void *out;
+    float *lse, *part;  // part: [slot][8 * NT rows][D + 2]
+    int64_t q_token_stride, q_head_stride;
+    float scale_log2;   // softmax scale * log2(e)
+    int64_t slots;      // of `part`
+    int64_t capacity;   // tokens of a row of the block table
+    FastDiv block_steps, by_group, by_grid;  // step -> block, row -> query, steps -> pieces
+    AttJoin *join;      // [piece]
+    uint32_t *pieces;   // how many there are
+    int32_t q_heads, group, causal, grid;
+};
+
+// How the line of steps is cut.  `padded`: every item begins a piece of its own (short lines: no item is split for nothing).
+struct AttCut {
+    uint32_t total;  // steps of the line
+    uint32_t per;    // steps of a piece
+    bool padded;
+};
+
+template <int NT>
+__device__ __forceinline__ int att_tiles(const AttArgs &a, const KvSeq &s) {
+    return (s.rows * a.group + NT * 8 - 1) / (NT * 8);
+}
+// steps of row tile `tile`: up to the last position that its last row sees
+template <int NT>
+__device__ __forceinline__ uint32_t att_steps(const AttArgs &a, const KvSeq &s, int tile) {
+    const int last = min(s.rows - 1, (int)fastdiv((uint32_t)((tile + 1) * NT * 8 - 1), a.by_group));
+    return (uint32_t)(kv_end(s, last, a.causal != 0) + 15) >> 4;
+}
+// places that an item takes on the line; one without a step has its place too, and is written there
+__device__ __forceinline__ uint32_t att_span(const AttCut &cut, uint32_t n) {
+    static_assert(kAttMinPiece == 16, "pieces of a padded line");
+    n = max(n, 1u);
+    return cut.padded ? (n + 15) & ~15u : n;
+}
+
+// steps of all tiles of a request, for one head
+template <int NT>
+__device__ __forceinline__ uint32_t att_request_steps(const AttArgs &a, const KvSeq &s, const AttCut &cut) {
+    uint32_t n = 0;
+    const int tiles = att_tiles<NT>(a, s);
+    for (int i = 0; i < tiles; ++i) n += att_span(cut, att_steps<NT>(a, s, i));
+    return n;
+}
+
+// Every warp walks the requests for itself, one per lane and 32 at a time; `first` is this lane's of the first 32.
+__device__ __forceinline__ KvSeq att_lane_seq(const AttArgs &a, const KvSeq &first, int base) {
+    const int b = base + (threadIdx.x & 31);
+    if (base == 0) return first;
+    return b < a.t.batch ? kv_seq(a.t, a.capacity, b) : KvSeq{0, 0, 0, 0};
+}
+
+// The whole line, over all requests and heads.  The host admits only calls whose line stays below 2^31 steps; row offsets
+// that decrease can make it longer, and then nothing is on it.
+template <int NT>
+__device__ __forceinline__ uint32_t att_total(const AttArgs &a, const KvSeq &first, const AttCut &cut) {
+    uint64_t n = 0;
+    for (int base = 0; base < a.t.batch; base += 32) n += att_request_steps<NT>(a, att_lane_seq(a, first, base), cut);
+    n = __reduce_add_sync(0xffffffffu, (uint32_t)(n & 0xffffu)) + ((uint64_t)__reduce_add_sync(0xffffffffu, (uint32_t)min(n >> 16, (uint64_t)0xffffffu)) << 16);
+    n *= (uint32_t)a.c.heads;
+    return n < 0x80000000ull ? (uint32_t)n : 0;
+}
+
+template <int NT>
+__device__ __forceinline__ AttCut att_cut(const AttArgs &a, const KvSeq &first) {
+    AttCut cut{0, 0, false};
+    cut.total = att_total<NT>(a, first, cut);
+    cut.per = fastdiv(cut.total + a.grid - 1, a.by_grid);
+    if (cut.per <= kAttMinPiece) {
+        cut.per = kAttMinPiece;
+        cut.padded = true;
+        cut.total = att_total<NT>(a, first, cut);
+    }
+    return cut;
+}
+
+struct AttItem {
+    KvSeq s;
+    int b, tile, head;
+    uint32_t begin, steps, span;  // first step on the line; real steps; places on the line
+};
+
+__device__ __forceinline__ uint32_t warp_inclusive(uint32_t v) {
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t u = __shfl_up_sync(0xffffffffu, v, o);
+        if ((threadIdx.x & 31) >= o) v += u;
+    }
+    return v;
+}
+
+// What request weigh(seq) of every request sums up to `pos`: the request, its KvSeq and the sum in front of it, in all lanes.
+template <class F>
+__device__ __forceinline__ int att_locate(const AttArgs &a, const KvSeq &first, uint32_t pos, F weigh, KvSeq &s, uint32_t &begin) {
+    uint32_t run = 0;
+    for (int base = 0; base < a.t.batch; base += 32) {
+        const KvSeq q = att_lane_seq(a, first, base);
+        const uint32_t n = weigh(q), upto = run + warp_inclusive(n);
+        const uint32_t hit = __ballot_sync(0xffffffffu, pos < upto);
+        if (hit) {
+            const int src = __ffs(hit) - 1;
+            s.first_row = __shfl_sync(0xffffffffu, q.first_row, src);
+            s.rows = __shfl_sync(0xffffffffu, q.rows, src);
+            s.len = __shfl_sync(0xffffffffu, q.len, src);
+            s.start = __shfl_sync(0xffffffffu, q.start, src);
+            begin = __shfl_sync(0xffffffffu, upto - n, src);
+            return base + src;
+        }
+        run = __shfl_sync(0xffffffffu, upto, 31);
+    }
+    return -1;
+}
+
+// The item that holds position `pos` of the line.
+template <int NT>
+__device__ __forceinline__ AttItem att_find(const AttArgs &a, const AttCut &cut, const KvSeq &first, uint32_t pos) {
+    AttItem it;
+    const uint32_t heads = (uint32_t)a.c.heads;
+    it.b = att_locate(a, first, pos, [&](const KvSeq &q) { return att_request_steps<NT>(a, q, cut) * heads; }, it.s, it.begin);
+    const int tiles = it.b < 0 ? 0 : att_tiles<NT>(a, it.s);
+    for (it.tile = 0; it.tile < tiles; ++it.tile) {
+        it.steps = att_steps<NT>(a, it.s, it.tile);
+        it.span = att_span(cut, it.steps);
+        if (pos < it.begin + it.span * heads) break;
+        it.begin += it.span * heads;
+    }
+    it.head = heads == 1 || it.span == 0 ? 0 : (int)((pos - it.begin) / it.span);
+    it.begin += it.head * it.span;
+    return it;
+}
+
+template <int D>
+struct AttShape {
+    static constexpr int HALVES = D / 64;              // 16-byte pieces of a key row per lane
+    static constexpr int VB = D / 8 < 16 ? D / 8 : 16; // bytes of a piece of a value row
+    static constexpr int VP = D / 8 / VB;              // such pieces per lane
+    static constexpr int STAGE = 16 * D * 2;           // bytes of a step: keys, then values
+    static constexpr int STAGES = D == 64 ? 6 : D == 128 ? 4 : 2;  // an even number: two steps are computed at a time
+};
+
+// two codes in the low (H = 0) or high half of a word -> f16x2
+template <bool INT8, int H>
+__device__ __forceinline__ uint32_t code_pair(uint32_t w) {
+    if constexpr (INT8) return sub2<CTB_F16>(__byte_perm(w, 0x64646464u, H ? 0x4342 : 0x4140), 0x64806480u);  // 1024 + (code ^ 128) - 1152
+    else return f16x2_from_e4m3x2(H ? w >> 16 : w);
+}
+template <bool INT8>
+__device__ __forceinline__ uint32_t code_word(uint32_t w) {
+    return INT8 ? w ^ 0x80808080u : w;
+}
+
+// Blocks that an SM holds: what shared memory (head size 256) and registers (two row tiles at 128) leave room for.
+__host__ __device__ constexpr int att_blocks(int head_dim, int nt) { return head_dim == 256 || (head_dim == 128 && nt == 2) ? 2 : 3; }
+
+template <int DT, bool INT8, int D, int NT>
+__global__ void __launch_bounds__(kAttThreads, att_blocks(D, NT)) kv_attention_kernel(const __grid_constant__ AttArgs a) {
+    using S = AttShape<D>;
+    constexpr int ROWS = NT * 8, MT = D / 16;
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ float s_m[kAttWarps][ROWS], s_l[kAttWarps][ROWS];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+    const KvSeq first = lane < a.t.batch ? kv_seq(a.t, a.capacity, lane) : KvSeq{0, 0, 0, 0};
+    grid_next();
+    const AttCut cut = att_cut<NT>(a, first);
+    if (blockIdx.x == 0 && threadIdx.x == 0) *a.pieces = (cut.total + cut.per - 1) / cut.per;
+    const uint32_t ring = smem_u32(smem) + warp * (S::STAGES * S::STAGE);
+    const int block_steps = a.c.block_size >> 4;
+    // this lane's pieces of a step: key rows g and g + 8, value rows 2t, 2t + 1, 2t + 8, 2t + 9
+    const int64_t k_lane = g * a.c.k_token_stride + t * 16, v_lane = 2 * t * a.c.v_token_stride + g * S::VB;
+
+    for (uint32_t piece = blockIdx.x; (uint64_t)piece * cut.per < cut.total; piece += a.grid) {
+        const uint32_t p0 = piece * cut.per, p1 = min(cut.total, p0 + cut.per);
+        bool open = false;  // an item begins here and ends behind the piece
+        for (uint32_t pos = p0; pos < p1;) {
+            const AttItem it = att_find<NT>(a, cut, first, pos);
+            if (it.b < 0 || pos - it.begin >= it.span) break;  // (not with row offsets in order)
+            const KvSeq sq = it.s;
+            const int steps = (int)it.steps, s0 = (int)(pos - it.begin), s1 = min(steps, (int)(p1 - it.begin));
+            pos = min(p1, it.begin + it.span);
+            // this warp's steps: s0 + warp, + 4, ...; what has to be known of 32 of them at a time, one per lane
+            const int mine = s1 - s0 > warp ? (s1 - s0 - warp + kAttWarps - 1) / kAttWarps : 0;
+            const int32_t *table = a.t.block_table + (int64_t)it.b * a.t.table_stride;
+            auto look_up = [&](int j) { return j < mine ? __ldg(table + fastdiv((uint32_t)(s0 + warp + j * kAttWarps), a.block_steps)) : -1; };
+            int page_next = look_up(lane);
+            const int rows = sq.rows * a.group, row0 = it.tile * ROWS;
+            const int last_end = kv_end(sq, min(sq.rows - 1, (int)fastdiv((uint32_t)(row0 + ROWS - 1), a.by_group)), a.causal != 0);
+            const int first_end = kv_end(sq, fastdiv((uint32_t)row0, a.by_group), a.causal != 0);
+
+            // query rows: lane (g, t) has row g of every tile of eight, elements 16 t .. 16 t + 15 of every 64
+            uint4 qraw[NT][D / 32];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                const int r = row0 + n * 8 + g, i = (int)fastdiv((uint32_t)r, a.by_group);
+                const bool in = r < rows;
+                const uint16_t *qr = (const uint16_t *)a.q + (int64_t)(sq.first_row + i) * a.q_token_stride + (int64_t)(it.head * a.group + r - i * a.group) * a.q_head_stride;
+#pragma unroll
+                for (int k = 0; k < D / 32; ++k) qraw[n][k] = in ? __ldg((const uint4 *)(qr + (k >> 1) * 64 + t * 16 + (k & 1) * 8)) : make_uint4(0, 0, 0, 0);
+            }
+            // for the 32 steps that are fetched, then for those that are computed: key and value scale; which blocks exist
+            float ks_next = 0.0f, vs_next = 1.0f, ks = 0.0f, lv = 0.0f, iv = 0.0f;
+            uint32_t ok_next = 0, ok = 0, some = 0;
+            const int pairs = (mine + 1) & ~1;  // two steps at a time; a missing second one reads as zeros and is masked
+            int issued = 0;
+            uint32_t put = 0;
+            const uint8_t *k0 = (const uint8_t *)a.c.k + (int64_t)it.head * a.c.k_head_stride + k_lane;
+            const uint8_t *v0 = (const uint8_t *)a.c.v + (int64_t)it.head * a.c.v_head_stride + v_lane;
+            int64_t k_at = 0, v_at = 0;  // of this lane's step
+            auto fetch = [&]() {
+                if (issued < pairs) {
+                    if ((issued & 31) == 0) {
+                        const bool there = (uint32_t)page_next < (uint32_t)a.c.num_blocks;  // (a number below zero is a large one)
+                        ok_next = __ballot_sync(0xffffffffu, there);
+                        const int64_t page = there ? page_next : 0;
+                        const uint32_t step = s0 + warp + (issued + lane) * kAttWarps;
+                        const int slot = (int)(step - fastdiv(step, a.block_steps) * block_steps) * 16;
+                        k_at = page * a.c.k_block_stride + slot * a.c.k_token_stride;
+                        v_at = page * a.c.v_block_stride + slot * a.c.v_token_stride;
+                        ks_next = __ldg(a.c.k_scale + page * a.c.heads + it.head);
+                        vs_next = __ldg(a.c.v_scale + page * a.c.heads + it.head);
+                        page_next = look_up(issued + 32 + lane);
+                    }
+                    const uint8_t *kp = k0 + __shfl_sync(0xffffffffu, k_at, issued & 31), *vp = v0 + __shfl_sync(0xffffffffu, v_at, issued & 31);
+                    // tokens of the step that any row sees; the others read as zeros
+                    const int seen = (ok_next >> (issued & 31)) & 1 ? last_end - (s0 + warp + issued * kAttWarps) * 16 : 0;
+                    const uint32_t dst = ring + put + lane * 16, vdst = ring + put + 16 * D + lane * S::VB;
+                    const int64_t k8 = 8 * a.c.k_token_stride, v1 = a.c.v_token_stride, v8 = 8 * a.c.v_token_stride;
+                    if (seen >= 16) {
+#pragma unroll
+                        for (int r = 0; r < 2; ++r)
+#pragma unroll
+                            for (int h = 0; h < S::HALVES; ++h) cp_async16(dst + (r * S::HALVES + h) * 512, kp + r * k8 + h * 64);
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+#pragma unroll
+                            for (int c = 0; c < S::VP; ++c) {
+                                const uint8_t *src = vp + (r & 1) * v1 + (r >> 1) * v8 + c * 128;
+                                if constexpr (S::VB == 16) cp_async16(vdst + (r * S::VP + c) * 512, src);
+                                else cp_async8(vdst + r * 256, src);
+                            }
+                    } else {
+#pragma unroll
+                        for (int r = 0; r < 2; ++r)
+#pragma unroll
+                            for (int h = 0; h < S::HALVES; ++h)
+                                cp_async16_some(dst + (r * S::HALVES + h) * 512, kp + r * k8 + h * 64, g + 8 * r < seen ? 16 : 0);
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+#pragma unroll
+                            for (int c = 0; c < S::VP; ++c) {
+                                const uint8_t *src = vp + (r & 1) * v1 + (r >> 1) * v8 + c * 128;
+                                const bool in = 2 * t + (r & 1) + (r >> 1) * 8 < seen;
+                                if constexpr (S::VB == 16) cp_async16_some(vdst + (r * S::VP + c) * 512, src, in ? 16 : 0);
+                                else cp_async8_some(vdst + r * 256, src, in ? 8 : 0);
+                            }
+                    }
+                }
+                ++issued;
+                put = put == (S::STAGES - 1) * S::STAGE ? 0 : put + S::STAGE;
+                cp_async_commit();
+            };
+#pragma unroll 1
+            for (int i = 0; i < S::STAGES; ++i) fetch();
+
+            uint32_t qf[NT][D / 16][2];
+            float f[NT][2];   // score factors of rows 2t, 2t + 1: softmax scale * log2 e * the row's power of two
+            int end[NT][2];   // positions that rows 2t, 2t + 1 see
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                uint32_t most = 0;  // as integers the absolute values order like the numbers, with infinity and NaN on top
+#pragma unroll
+                for (int k = 0; k < D / 32; ++k)
+                    most = __vmaxu2(most, __vmaxu2(__vmaxu2(qraw[n][k].x & 0x7fff7fffu, qraw[n][k].y & 0x7fff7fffu),
+                                                   __vmaxu2(qraw[n][k].z & 0x7fff7fffu, qraw[n][k].w & 0x7fff7fffu)));
+                most = __vmaxu2(most, __shfl_xor_sync(0xffffffffu, most, 1));
+                most = __vmaxu2(most, __shfl_xor_sync(0xffffffffu, most, 2));
+                const float top = half_f32<DT>(max(most & 0xffffu, most >> 16));
+                const int e = max((int)(__float_as_uint(top) >> 23), 8);
+                const float up = __uint_as_float((uint32_t)(261 - e) << 23);  // the largest element comes to [128, 256)
+#pragma unroll
+                for (int k = 0; k < D / 16; ++k) {  // k = 4 h + i: elements 16 t + 4 i .. + 3 of half h
+                    const uint4 v = qraw[n][k >> 1];
+                    const uint32_t x0 = k & 1 ? v.z : v.x, x1 = k & 1 ? v.w : v.y;
+                    qf[n][k][0] = pack_f16x2(half_f32<DT>(x0 & 0xffffu) * up, half_f32<DT>(x0 >> 16) * up);
+                    qf[n][k][1] = pack_f16x2(half_f32<DT>(x1 & 0xffffu) * up, half_f32<DT>(x1 >> 16) * up);
+                }
+                const float own = a.scale_log2 * __uint_as_float((uint32_t)max(e - 7, 1) << 23);
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {  // lane 4 (2t + i) has row 2t + i
+                    f[n][i] = __shfl_sync(0xffffffffu, own, (2 * t + i) * 4);
+                    const int rr = row0 + n * 8 + 2 * t + i;
+                    end[n][i] = rr < rows ? kv_end(sq, fastdiv((uint32_t)rr, a.by_group), a.causal != 0) : 0;
+                }
+            }
+
+            float o[NT][MT][4], m[NT][2], l[NT][2];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                m[n][0] = m[n][1] = -3.402823466e38f;
+                l[n][0] = l[n][1] = 0.0f;
+#pragma unroll
+                for (int j = 0; j < MT; ++j) o[n][j][0] = o[n][j][1] = o[n][j][2] = o[n][j][3] = 0.0f;
+            }
+
+            uint32_t get = 0;
+            for (int j = 0; j < pairs; j += 2) {
+                if ((j & 31) == 0) {  // (those after these are looked up later than this)
+                    // a zero scale has no logarithm: 2^-120 stands for it in the weights, and the values of its block are left out
+                    const float vsafe = vs_next < 0x1p-120f ? 0x1p-120f : vs_next;
+                    some = __ballot_sync(0xffffffffu, vs_next != 0.0f);
+                    ks = ks_next, ok = ok_next, lv = log2f(vsafe), iv = 1.0f / vsafe;
+                }
+                cp_async_wait<S::STAGES - 2>();
+                const uint8_t *st0 = smem + warp * (S::STAGES * S::STAGE) + get;
+                float sc[2][NT][4];
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const uint8_t *st = st0 + u * S::STAGE;
+#pragma unroll
+                    for (int h = 0; h < S::HALVES; ++h) {
+                        const uint4 ka = *(const uint4 *)(st + h * 512 + lane * 16), kb = *(const uint4 *)(st + (S::HALVES + h) * 512 + lane * 16);
+                        const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const uint32_t xa = code_word<INT8>(wa[i]), xb = code_word<INT8>(wb[i]);
+                            const uint32_t a0 = code_pair<INT8, 0>(xa), a1 = code_pair<INT8, 0>(xb), a2 = code_pair<INT8, 1>(xa), a3 = code_pair<INT8, 1>(xb);
+#pragma unroll
+                            for (int n = 0; n < NT; ++n) {
+                                if (h == 0 && i == 0) mma16816_first<CTB_F16>(sc[u][n], a0, a1, a2, a3, qf[n][0][0], qf[n][0][1]);
+                                else mma16816<CTB_F16>(sc[u][n], a0, a1, a2, a3, qf[n][h * 4 + i][0], qf[n][h * 4 + i][1]);
+                            }
+                        }
+                    }
+                }
+                bool over = false;
+                float ivj[2];
+                uint32_t keep[2];
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const float ksj = __shfl_sync(0xffffffffu, ks, (j & 31) + u), lvj = __shfl_sync(0xffffffffu, lv, (j & 31) + u);
+                    ivj[u] = __shfl_sync(0xffffffffu, iv, (j & 31) + u);
+                    const bool there = (ok >> ((j & 31) + u)) & 1;
+                    keep[u] = (some >> ((j & 31) + u)) & 1 ? 0xffffffffu : 0;
+                    const int tok = (s0 + warp + (j + u) * kAttWarps) * 16;
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) sc[u][n][i] = fmaf(sc[u][n][i], ksj * f[n][i & 1], lvj);
+                        if (tok + 16 > first_end || !there) {
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                if (!there || tok + g + (i >> 1) * 8 >= end[n][i & 1]) sc[u][n][i] = -INFINITY;
+                        }
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) over |= sc[u][n][i] > m[n][i & 1] + 8.0f;
+                    }
+                }
+                if (__any_sync(0xffffffffu, over)) {
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            float x = fmaxf(fmaxf(sc[0][n][i], sc[0][n][i + 2]), fmaxf(sc[1][n][i], sc[1][n][i + 2]));
+#pragma unroll
+                            for (int s = 4; s < 32; s <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, s));
+                            const float mn = fmaxf(m[n][i], x), down = ex2(m[n][i] - mn);
+                            m[n][i] = mn;
+                            l[n][i] *= down;
+#pragma unroll
+                            for (int k = 0; k < MT; ++k) {
+                                o[n][k][i] *= down;
+                                o[n][k][i + 2] *= down;
+                            }
+                        }
+                }
+                uint32_t pb[2][NT][2];
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            sc[u][n][i] = ex2(sc[u][n][i] - m[n][i & 1]);
+                            l[n][i & 1] = fmaf(sc[u][n][i], ivj[u], l[n][i & 1]);
+                        }
+                        pb[u][n][0] = movmatrix_trans(pack_f16x2(sc[u][n][0], sc[u][n][1]) & keep[u]);
+                        pb[u][n][1] = movmatrix_trans(pack_f16x2(sc[u][n][2], sc[u][n][3]) & keep[u]);
+                    }
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const uint8_t *sv = st0 + u * S::STAGE + 16 * D + lane * S::VB;
+#pragma unroll
+                    for (int c = 0; c < S::VP; ++c) {
+                        uint32_t v[4][S::VB / 4];
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            if constexpr (S::VB == 16) {
+                                const uint4 x = *(const uint4 *)(sv + (r * S::VP + c) * 512);
+                                v[r][0] = code_word<INT8>(x.x), v[r][1] = code_word<INT8>(x.y), v[r][2] = code_word<INT8>(x.z), v[r][3] = code_word<INT8>(x.w);
+                            } else {
+                                const uint2 x = *(const uint2 *)(sv + r * 256);
+                                v[r][0] = code_word<INT8>(x.x), v[r][1] = code_word<INT8>(x.y);
+                            }
+                        }
+#pragma unroll
+                        for (int k = 0; k < S::VB / 2; ++k) {  // d = 2k and 2k + 1 of the lane's bytes are rows g and g + 8 of a tile
+                            const uint32_t sel = k & 1 ? 0x7362 : 0x5140;
+                            const uint32_t x = __byte_perm(v[0][k >> 1], v[1][k >> 1], sel), y = __byte_perm(v[2][k >> 1], v[3][k >> 1], sel);
+                            const uint32_t a0 = code_pair<INT8, 0>(x), a1 = code_pair<INT8, 1>(x), a2 = code_pair<INT8, 0>(y), a3 = code_pair<INT8, 1>(y);
+#pragma unroll
+                            for (int n = 0; n < NT; ++n) mma16816<CTB_F16>(o[n][c * (S::VB / 2) + k], a0, a1, a2, a3, pb[u][n][0], pb[u][n][1]);
+                        }
+                    }
+                }
+                get = get == (S::STAGES - 2) * S::STAGE ? 0 : get + 2 * S::STAGE;
+                fetch();
+                fetch();
+            }
+            cp_async_wait<0>();
+
+            // the four warps' results: sums over the lanes of a row, then over the warps in order
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+#pragma unroll
+                    for (int s = 4; s < 32; s <<= 1) l[n][i] += __shfl_xor_sync(0xffffffffu, l[n][i], s);
+                    if (g == 0) {
+                        s_m[warp][n * 8 + 2 * t + i] = m[n][i];
+                        s_l[warp][n * 8 + 2 * t + i] = l[n][i];
+                    }
+                }
+            __syncthreads();  // (every ring is idle from here on: the sums go where it was)
+            float *so = reinterpret_cast<float *>(smem);
+            constexpr int OS = D + 4;
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int r = n * 8 + 2 * t + i;
+                    float top = s_m[0][r];
+#pragma unroll
+                    for (int w = 1; w < kAttWarps; ++w) top = fmaxf(top, s_m[w][r]);
+                    const float down = ex2(m[n][i] - top);
+                    float *row = so + ((size_t)warp * ROWS + r) * OS;
+#pragma unroll
+                    for (int c = 0; c < S::VP; ++c)
+#pragma unroll
+                        for (int k = 0; k < S::VB / 2; ++k) {
+                            const float(&x)[4] = o[n][c * (S::VB / 2) + k];
+                            *(float2 *)(row + c * 128 + g * S::VB + 2 * k) = make_float2(x[i] * down, x[i + 2] * down);
+                        }
+                }
+            __syncthreads();
+            const bool whole = s0 == 0 && s1 == steps;
+            const int64_t slot = cut.padded ? piece : 2 * (int64_t)piece + (p0 < it.begin ? 1 : 0);
+            float *part = a.part + slot * ROWS * (D + 2);
+            for (int i = threadIdx.x; i < ROWS * (D / 2); i += kAttThreads) {
+                const int r = i / (D / 2), d = (i % (D / 2)) * 2;
+                if (row0 + r >= rows) break;
+                float top = s_m[0][r], sum = 0.0f;
+#pragma unroll
+                for (int w = 1; w < kAttWarps; ++w) top = fmaxf(top, s_m[w][r]);
+#pragma unroll
+                for (int w = 0; w < kAttWarps; ++w) sum += s_l[w][r] * ex2(s_m[w][r] - top);
+                float2 v = make_float2(0.0f, 0.0f);
+#pragma unroll
+                for (int w = 0; w < kAttWarps; ++w) {
+                    const float2 x = *(const float2 *)(so + ((size_t)w * ROWS + r) * OS + d);
+                    v.x += x.x, v.y += x.y;
+                }
+                if (whole) {
+                    const int qi = (int)fastdiv((uint32_t)(row0 + r), a.by_group);
+                    const int64_t row = (int64_t)(sq.first_row + qi) * a.q_heads + it.head * a.group + row0 + r - qi * a.group;
+                    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;  // nothing seen: zeros
+                    store_half2<DT>((uint16_t *)a.out + row * D + d, v.x * inv, v.y * inv);
+                    if (d == 0) a.lse[row] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
+                } else if (slot < a.slots) {  // (row offsets that decrease may ask for more than there are)
+                    *(float2 *)(part + r * (D + 2) + d) = v;
+                    if (d == 0) *(float2 *)(part + r * (D + 2) + D) = make_float2(top, sum);
+                }
+            }
+            if (threadIdx.x == 0 && s1 < steps && it.begin >= p0 && piece < a.slots) {
+                const int qi = (int)fastdiv((uint32_t)row0, a.by_group);
+                a.join[piece] = AttJoin{(int64_t)(sq.first_row + qi) * a.q_heads + it.head * a.group, slot, (it.begin + (uint32_t)steps - 1) / cut.per,
+                                        min(ROWS, rows - row0), row0 - qi * a.group, cut.padded};
+                open = true;
+            }
+            __syncthreads();  // the next item's copies go where the sums are
+        }
+        if (threadIdx.x == 0 && !open && piece < a.slots) a.join[piece].last = 0;
+    }
+    // rows in front of the first request and behind the last one: zeros
+    const int64_t lo = a.t.batch > 0 ? min(max((int64_t)a.t.query_start[0], (int64_t)0), a.t.tokens) : 0;
+    const int64_t hi = a.t.batch > 0 ? min(max((int64_t)a.t.query_start[a.t.batch], lo), a.t.tokens) : 0;
+    for (int64_t i = blockIdx.x; i < lo + a.t.tokens - hi; i += gridDim.x) {
+        const int64_t row = (i < lo ? i : hi + i - lo) * a.q_heads;
+        for (int j = threadIdx.x; j < a.q_heads * (D / 2); j += kAttThreads) store_half2<DT>((uint16_t *)a.out + row * D + 2 * j, 0.0f, 0.0f);
+        for (int j = threadIdx.x; j < a.q_heads; j += kAttThreads) a.lse[row + j] = -INFINITY;
+    }
+}
+
+// Joins what the pieces of an item left in scratch: block c takes the item that begins in piece c and ends behind it.
+constexpr int kJoinWarps = 16;
+
+template <int DT, int D, int NT>
+__global__ void __launch_bounds__(kJoinWarps * 32) kv_attention_join_kernel(const __grid_constant__ AttArgs a) {
+    constexpr int ROWS = NT * 8, E = D / 32, B = D == 256 ? 4 : 8;  // B: pieces in flight per warp
+    __shared__ float s_v[kJoinWarps][D], s_top[kJoinWarps], s_sum[kJoinWarps];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    grid_wait();
+    const uint32_t pieces = (uint32_t)min((int64_t)__ldcg(a.pieces), a.slots);
+    for (uint32_t c = blockIdx.x; c < pieces; c += gridDim.x) {
+        const uint32_t last = __ldcg(&a.join[c].last);
+        if (last == 0) continue;
+        const AttJoin it = a.join[c];
+        const int n = it.rows;
+        // all warps on the rows: 16 / (n rounded up to a power of two) of them on each, every one with its share of the pieces
+        const int log_rows = n <= 1 ? 0 : 32 - __clz(n - 1), log_warps = 4 - log_rows, r = warp & ((1 << log_rows) - 1);
+        float top = -3.402823466e38f, sum = 0.0f, v[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) v[e] = 0.0f;
+        if (r < n) {
+            for (uint32_t p0 = c + (warp >> log_rows); p0 <= last; p0 += B << log_warps) {
+                float x[B][E];
+                float2 ml[B];
+#pragma unroll
+                for (int i = 0; i < B; ++i) {
+                    const uint32_t p = p0 + ((uint32_t)i << log_warps);
+                    ml[i] = make_float2(-INFINITY, 0.0f);
+#pragma unroll
+                    for (int e = 0; e < E; ++e) x[i][e] = 0.0f;
+                    const int64_t slot = p == c ? it.slot : it.padded ? p : 2 * (int64_t)p;
+                    if (p <= last && slot < a.slots) {
+                        const float *part = a.part + (slot * ROWS + r) * (D + 2);
+                        ml[i] = __ldcg((const float2 *)(part + D));
+#pragma unroll
+                        for (int e = 0; e < E; e += 2) *(float2 *)&x[i][e] = __ldcg((const float2 *)(part + lane * E + e));
+                    }
+                }
+                float mn = top;
+#pragma unroll
+                for (int i = 0; i < B; ++i) mn = fmaxf(mn, ml[i].x);
+                const float w0 = ex2(top - mn);
+                sum *= w0;
+#pragma unroll
+                for (int e = 0; e < E; ++e) v[e] *= w0;
+#pragma unroll
+                for (int i = 0; i < B; ++i) {
+                    const float w = ex2(ml[i].x - mn);
+                    sum = fmaf(ml[i].y, w, sum);
+#pragma unroll
+                    for (int e = 0; e < E; ++e) v[e] = fmaf(x[i][e], w, v[e]);
+                }
+                top = mn;
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < E; ++e) s_v[warp][lane * E + e] = v[e];
+        if (lane == 0) s_top[warp] = top, s_sum[warp] = sum;
+        __syncthreads();
+        for (int i = threadIdx.x; i < n * (D / 2); i += kJoinWarps * 32) {
+            const int q = i / (D / 2), d = (i % (D / 2)) * 2;
+            float all = -3.402823466e38f, total = 0.0f, x0 = 0.0f, x1 = 0.0f;
+            for (int w = 0; w < 1 << log_warps; ++w) all = fmaxf(all, s_top[(w << log_rows) + q]);
+            for (int w = 0; w < 1 << log_warps; ++w) {
+                const int k = (w << log_rows) + q;
+                const float down = ex2(s_top[k] - all);
+                total = fmaf(s_sum[k], down, total);
+                x0 = fmaf(s_v[k][d], down, x0);
+                x1 = fmaf(s_v[k][d + 1], down, x1);
+            }
+            const int rr = it.first + q, qi = (int)fastdiv((uint32_t)rr, a.by_group);
+            const int64_t row = it.row + (int64_t)qi * a.q_heads + rr - qi * a.group;
+            const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+            store_half2<DT>((uint16_t *)a.out + row * D + d, x0 * inv, x1 * inv);
+            if (d == 0) a.lse[row] = total == 0.0f ? -INFINITY : (all + log2f(total)) * 0.6931471805599453f;
+        }
+        __syncthreads();
+    }
+}
+
+// ---------------------------------------------------------------- host side
+
+static int64_t att_items(const ctb_kv_cache &c, const ctb_kv_batch &t, int group, int rows) {
+    return (int64_t)c.heads * ((t.tokens * group + rows - 1) / rows + t.batch);  // a tile for every `rows` query rows, and one more per request
+}
+
+static int att_nt(const ctb_kv_cache &c, const ctb_kv_batch &t, int group) {
+    // two tiles of eight rows per step where a request has more than eight rows on average; head size 256 has registers for one
+    return c.head_dim <= 128 && t.tokens * group > 8 * (int64_t)t.batch ? 2 : 1;
+}
+
+static int att_grid(int head_dim, int nt) { return sm_count() * att_blocks(head_dim, nt); }
+
+bool kv_attention_takes(const ctb_kv_cache &c, const ctb_kv_batch &t, int q_heads, const void *q, int64_t q_token_stride, int64_t q_head_stride, const void *out) {
+    const int64_t strides = c.k_block_stride | c.k_head_stride | c.k_token_stride | c.v_block_stride | c.v_head_stride | c.v_token_stride;
+    return (c.head_dim == 64 || c.head_dim == 128 || c.head_dim == 256) && c.num_blocks > 0 && c.block_size % 16 == 0 && strides % 16 == 0 && aligned16(c.k) && aligned16(c.v) &&
+           // positions on the line of steps are 32-bit numbers
+           (double)att_items(c, t, q_heads / c.heads, 8) * ((double)t.table_width * c.block_size / 16 + 16) < 2147483648.0 &&
+           aligned16(q) && (q_token_stride | q_head_stride) % 8 == 0 && ((uintptr_t)out & 3) == 0;
+}
+
+// Scratch: 32 bytes, what is to be joined, the parts.  A slot per short item, two per piece of a long line.
+static int64_t att_slots(const ctb_kv_cache &c, const ctb_kv_batch &t, int group, int nt) {
+    return att_items(c, t, group, 8 * nt) + 2 * (int64_t)att_grid(c.head_dim, nt);
+}
+
+int64_t kv_attention_workspace(const ctb_kv_cache &c, const ctb_kv_batch &t, int q_heads) {
+    const int group = q_heads / c.heads, nt = att_nt(c, t, group);
+    return 32 + att_slots(c, t, group, nt) * ((int64_t)sizeof(AttJoin) + 8 * nt * (c.head_dim + 2) * 4);
+}
+
+template <int DT, bool INT8, int D, int NT>
+static int att_launch(const AttArgs &a, cudaStream_t st) {
+    auto kernel = kv_attention_kernel<DT, INT8, D, NT>;
+    constexpr size_t ring = (size_t)kAttWarps * AttShape<D>::STAGES * AttShape<D>::STAGE, sums = (size_t)kAttWarps * NT * 8 * (D + 4) * 4;
+    constexpr size_t bytes = ring > sums ? ring : sums;
+    static std::atomic<bool> ready[64];
+    int rc = allow_smem(kernel, bytes, ready);
+    if (rc) return rc;
+    kernel<<<a.grid, kAttThreads, bytes, st>>>(a);
+    rc = after_launch("kv_attention_kernel");
+    // no request is longer than the shortest piece, and there is a block for each: nothing to join
+    if (rc || (a.capacity <= kAttMinPiece * 16 && att_items(a.c, a.t, a.group, NT * 8) <= a.grid)) return rc;
+    return launch_dependent("kv_attention_join_kernel", kv_attention_join_kernel<DT, D, NT>, dim3((unsigned)a.grid), kJoinWarps * 32, 0, st, a);
+}
+
+int kv_attention_launch(const ctb_kv_cache &c, const ctb_kv_batch &t, const void *q, int dtype, int64_t q_token_stride, int64_t q_head_stride, int q_heads,
+                        float softmax_scale, int causal, void *out, float *lse, void *workspace, cudaStream_t st) {
+    const int group = q_heads / c.heads, nt = att_nt(c, t, group);
+    AttArgs a;
+    a.c = c;
+    a.t = t;
+    a.q = q;
+    a.out = out;
+    a.lse = lse;
+    a.slots = att_slots(c, t, group, nt);
+    a.pieces = (uint32_t *)workspace;
+    a.join = (AttJoin *)((char *)workspace + 32);
+    a.part = (float *)(a.join + a.slots);
+    a.q_token_stride = q_token_stride;
+    a.q_head_stride = q_head_stride;
+    a.scale_log2 = softmax_scale * 1.4426950408889634f;
+    a.capacity = t.table_width * c.block_size;
+    a.grid = att_grid(c.head_dim, nt);
+    a.block_steps = make_fastdiv((uint32_t)(c.block_size / 16));
+    a.by_group = make_fastdiv((uint32_t)group);
+    a.by_grid = make_fastdiv((uint32_t)a.grid);
+    a.q_heads = q_heads;
+    a.group = group;
+    a.causal = causal;
+    auto go = [&](auto dt, auto i8) {
+        constexpr int DT = decltype(dt)::value;
+        constexpr bool I8 = decltype(i8)::value;
+        if (c.head_dim == 64) return nt == 1 ? att_launch<DT, I8, 64, 1>(a, st) : att_launch<DT, I8, 64, 2>(a, st);
+        if (c.head_dim == 128) return nt == 1 ? att_launch<DT, I8, 128, 1>(a, st) : att_launch<DT, I8, 128, 2>(a, st);
+        return att_launch<DT, I8, 256, 1>(a, st);
+    };
+    using B = std::integral_constant<int, CTB_BF16>;
+    using H = std::integral_constant<int, CTB_F16>;
+    if (dtype == CTB_BF16) return c.dtype == CTB_I8 ? go(B{}, std::true_type{}) : go(B{}, std::false_type{});
+    return c.dtype == CTB_I8 ? go(H{}, std::true_type{}) : go(H{}, std::false_type{});
+}
+
+}  // namespace ctb

@@ -32,6 +32,7 @@ __device__ __forceinline__ float quotient_to_odd(float x, float s) {
 
 template <bool INT8>
 __device__ __forceinline__ uint8_t cache_code(float q) {
+    if (q != q) return 0;  // then the scale is an infinity or NaN: it alone marks the block, so that queries that do not see it stay clean
     if constexpr (INT8) return (uint8_t)(int8_t)(int)fminf(fmaxf(rintf(q), -128.0f), 127.0f);
     else return f32_to_e4m3(q);
 }
@@ -228,21 +229,28 @@ extern "C" int ctb_kv_cache_append(const ctb_kv_cache *c, const ctb_kv_batch *t,
     return after_launch("kv_append_kernel");
 }
 
-extern "C" int64_t ctb_kv_cache_attention_workspace_bytes(const ctb_kv_cache *, const ctb_kv_batch *, int32_t) { return 0; }
+extern "C" int64_t ctb_kv_cache_attention_workspace_bytes(const ctb_kv_cache *c, const ctb_kv_batch *t, int32_t q_heads) {
+    using namespace ctb;
+    if (kv_check(c, t, CTB_BF16) || q_heads < 1 || q_heads % c->heads || t->tokens == 0) return 0;
+    return kv_attention_workspace(*c, *t, q_heads);
+}
 
 extern "C" int ctb_kv_cache_attention(const ctb_kv_cache *c, const ctb_kv_batch *t, const void *q, int32_t dtype, int64_t q_token_stride,
                                       int64_t q_head_stride, int32_t q_heads, float softmax_scale, int32_t causal, void *out, float *lse,
                                       void *workspace, void *stream) {
     using namespace ctb;
-    (void)workspace;
     int rc = kv_check(c, t, dtype);
     if (rc) return rc;
     if (q_heads < 1 || q_heads % c->heads) return fail(CTB_EINVAL_SHAPE, "%d query heads are no multiple of %d cache heads", q_heads, c->heads);
     if (q_heads > 65535) return fail(CTB_EUNSUPPORTED, "too many heads");
     if (t->tokens == 0) return CTB_OK;
     if (!q || !out || !lse) return fail(CTB_EINVAL_NULL, "null queries or outputs");
-    const dim3 grid((unsigned)t->tokens, (unsigned)q_heads);
     const cudaStream_t st = as_stream(stream);
+    if (kv_attention_takes(*c, *t, q_heads, q, q_token_stride, q_head_stride, out)) {
+        if (!workspace) return fail(CTB_EINVAL_NULL, "null workspace");
+        return kv_attention_launch(*c, *t, q, dtype, q_token_stride, q_head_stride, q_heads, softmax_scale, causal, out, lse, workspace, st);
+    }
+    const dim3 grid((unsigned)t->tokens, (unsigned)q_heads);
 #define CTB_ATT(DT, I8) kv_attention_any_kernel<DT, I8><<<grid, kAnyWarps * 32, 0, st>>>(*c, *t, q, q_token_stride, q_head_stride, q_heads, softmax_scale, causal, out, lse)
     if (dtype == CTB_BF16) {
         if (c->dtype == CTB_I8) CTB_ATT(CTB_BF16, true);

@@ -36,4 +36,10 @@ __device__ __forceinline__ int64_t block_exclusive(int64_t mine, int64_t *tmp, i
 // host: what every entry point refuses
 int kv_check(const ctb_kv_cache *c, const ctb_kv_batch *t, int32_t dtype);
 
+// ctb_kv_attention.cu: the attention for few query rows per cache head; whether it takes a call, its scratch, the call
+bool kv_attention_takes(const ctb_kv_cache &c, const ctb_kv_batch &t, int q_heads, const void *q, int64_t q_token_stride, int64_t q_head_stride, const void *out);
+int64_t kv_attention_workspace(const ctb_kv_cache &c, const ctb_kv_batch &t, int q_heads);
+int kv_attention_launch(const ctb_kv_cache &c, const ctb_kv_batch &t, const void *q, int dtype, int64_t q_token_stride, int64_t q_head_stride, int q_heads,
+                        float softmax_scale, int causal, void *out, float *lse, void *workspace, cudaStream_t st);
+
 }  // namespace ctb

@@ -11,7 +11,7 @@ namespace ctb {
 // host: the opt-in to more than 48 KiB of dynamic shared memory, once per device (`ready`: one flag per device)
 template <class K>
 static int allow_smem(K kernel, size_t bytes, std::atomic<bool> (&ready)[64]) {
-    if (bytes <= 48 * 1024) return CTB_OK;
+    if (bytes <= 40 * 1024) return CTB_OK;  // the limit of 48 KiB counts static shared memory too
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return fail(CTB_ECUDA, "cudaGetDevice: %s", cudaGetErrorString(e));
@@ -45,12 +45,47 @@ static int launch_cluster(const char *what, void (*kernel)(P...), dim3 grid, uns
     return after_launch(what);
 }
 
+// host: the second kernel of a pair, set up while the first one still runs; the kernel calls grid_wait() before it touches
+// anything that an earlier kernel writes, or writes anything itself
+template <class... P, class... A>
+static int launch_dependent(const char *what, void (*kernel)(P...), dim3 grid, unsigned threads, size_t smem, cudaStream_t st, A... args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        return fail(CTB_ECUDA, "%s: %s", what, cudaGetErrorString(e));
+    }
+    return after_launch(what);
+}
+
 #ifdef __CUDACC__
+
+__device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void grid_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
 __device__ __forceinline__ uint32_t smem_u32(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async8(uint32_t dst, const void *src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
+}
+// the first n of 16 (8) bytes, then zeros
+__device__ __forceinline__ void cp_async16_some(uint32_t dst, const void *src, int n) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void cp_async8_some(uint32_t dst, const void *src, int n) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
 }
 __device__ __forceinline__ void st_shared16_zero(uint32_t dst) {
     asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(dst), "r"(0) : "memory");
@@ -120,15 +155,35 @@ __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
     asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
     return r;
 }
-// two e4m3 codes in the low 16 bits <-> two f16 in the same order
-__device__ __forceinline__ uint32_t e4m3x2_from_f16x2(uint32_t v) {
-    uint16_t r;
-    asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(r) : "r"(v));
-    return r;
-}
+// two e4m3 codes in the low 16 bits -> two f16 in the same order
 __device__ __forceinline__ uint32_t f16x2_from_e4m3x2(uint32_t v) {
     uint32_t r;
     asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"((uint16_t)v));
+    return r;
+}
+
+// the transpose of an 8 x 8 matrix of 16-bit values, held by a warp as the matrix instructions hold one
+__device__ __forceinline__ uint32_t movmatrix_trans(uint32_t v) {
+    uint32_t r;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+template <int DT>
+__device__ __forceinline__ float half_f32(uint32_t h) {
+    if constexpr (DT == CTB_BF16) return bf16_bits_to_f32(h);
+    else return __half2float(__ushort_as_half((unsigned short)h));
+}
+template <int DT>
+__device__ __forceinline__ void store_half2(uint16_t *p, float lo, float hi) {
+    uint32_t r;
+    if constexpr (DT == CTB_BF16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    *reinterpret_cast<uint32_t *>(p) = r;
+}
+// 2^x: two units in the last place, subnormal results are zero
+__device__ __forceinline__ float ex2(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
 
