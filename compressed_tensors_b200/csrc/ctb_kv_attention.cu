@@ -23,7 +23,7 @@
 // Work.  The steps of all (request, row tile, head) items form one line that is cut into equal pieces, one per
 // block, whatever the lengths are; a piece's parts of an item that other pieces share go to scratch as (O, m, sum), and the
 // second kernel joins them.  The warps of a block take every fourth step and join in shared memory.  Each warp keeps
-// kAttStages steps in flight with cp.async: a lane copies the pieces that it will itself read, so its own wait is enough.
+// several steps in flight with cp.async.
 #include <atomic>
 
 #include "ctb_fastdiv.h"
@@ -178,20 +178,32 @@ __device__ __forceinline__ AttItem att_find(const AttArgs &a, const AttCut &cut,
     return it;
 }
 
+// A step in shared memory: 16 key rows, then 16 value rows.  Rows are copied whole and in order, 16 bytes per lane (with a
+// warp instruction spread over many rows the cache was read a quarter slower), and land where the reads below find them without
+// two lanes of a phase in one bank:
+//   keys: lane (g, t) reads bytes 64 h + 16 t of rows g and g + 8: odd rows have their 64-byte halves exchanged;
+//   values: lane (g, t) reads D / 8 bytes at g of rows 2t, 2t + 1, 2t + 8, 2t + 9: the 16-byte pieces of a row are permuted by
+//   bits 1 and 2 of its number; rows of 64 bytes are also reordered, so that rows 2t fill whole lines.
 template <int D>
 struct AttShape {
-    static constexpr int HALVES = D / 64;              // 16-byte pieces of a key row per lane
-    static constexpr int VB = D / 8 < 16 ? D / 8 : 16; // bytes of a piece of a value row
-    static constexpr int VP = D / 8 / VB;              // such pieces per lane
-    static constexpr int STAGE = 16 * D * 2;           // bytes of a step: keys, then values
+    static constexpr int HALVES = D / 64;              // 64-byte parts of a key row
+    static constexpr int PIECES = D / 16, ROWS = 32 / PIECES;  // 16-byte pieces of a row; rows that a warp instruction copies
+    static constexpr int VB = D / 8 < 16 ? D / 8 : 16; // bytes of a value row that a lane reads at once
+    static constexpr int VP = D / 8 / VB;              // such reads per row
+    static constexpr int STAGE = 16 * D * 2;           // bytes of a step
     static constexpr int STAGES = D == 64 ? 6 : D == 128 ? 4 : 2;  // an even number: two steps are computed at a time
+    static __device__ __forceinline__ uint32_t key_at(int row, int piece) { return row * D + (piece ^ (D == 64 ? 0 : (row & 1) << 2)) * 16; }
+    static __device__ __forceinline__ uint32_t value_at(int row, int piece) {
+        if (D == 64) return ((row & ~3) | (row & 1) << 1 | (row >> 1 & 1)) * 64 + (piece ^ (row >> 1 & 2)) * 16;
+        return row * D + (piece ^ (row & 6)) * 16;
+    }
 };
 
 // two codes in the low (H = 0) or high half of a word -> f16x2
 template <bool INT8, int H>
 __device__ __forceinline__ uint32_t code_pair(uint32_t w) {
     if constexpr (INT8) return sub2<CTB_F16>(__byte_perm(w, 0x64646464u, H ? 0x4342 : 0x4140), 0x64806480u);  // 1024 + (code ^ 128) - 1152
-    else return f16x2_from_e4m3x2(H ? w >> 16 : w);
+    else return f16x2_from_e4m3x2<H>(w);
 }
 template <bool INT8>
 __device__ __forceinline__ uint32_t code_word(uint32_t w) {
@@ -214,8 +226,9 @@ __global__ void __launch_bounds__(kAttThreads, att_blocks(D, NT)) kv_attention_k
     if (blockIdx.x == 0 && threadIdx.x == 0) *a.pieces = (cut.total + cut.per - 1) / cut.per;
     const uint32_t ring = smem_u32(smem) + warp * (S::STAGES * S::STAGE);
     const int block_steps = a.c.block_size >> 4;
-    // this lane's pieces of a step: key rows g and g + 8, value rows 2t, 2t + 1, 2t + 8, 2t + 9
-    const int64_t k_lane = g * a.c.k_token_stride + t * 16, v_lane = 2 * t * a.c.v_token_stride + g * S::VB;
+    // what this lane copies of a step: piece c of rows r, r + ROWS, ...
+    const int copy_row = lane / S::PIECES, copy_piece = lane % S::PIECES;
+    const int64_t k_lane = copy_row * a.c.k_token_stride + copy_piece * 16, v_lane = copy_row * a.c.v_token_stride + copy_piece * 16;
 
     for (uint32_t piece = blockIdx.x; (uint64_t)piece * cut.per < cut.total; piece += a.grid) {
         const uint32_t p0 = piece * cut.per, p1 = min(cut.total, p0 + cut.per);
@@ -271,36 +284,28 @@ __global__ void __launch_bounds__(kAttThreads, att_blocks(D, NT)) kv_attention_k
                     const uint8_t *kp = k0 + __shfl_sync(0xffffffffu, k_at, issued & 31), *vp = v0 + __shfl_sync(0xffffffffu, v_at, issued & 31);
                     // tokens of the step that any row sees; the others read as zeros
                     const int seen = (ok_next >> (issued & 31)) & 1 ? last_end - (s0 + warp + issued * kAttWarps) * 16 : 0;
-                    const uint32_t dst = ring + put + lane * 16, vdst = ring + put + 16 * D + lane * S::VB;
-                    const int64_t k8 = 8 * a.c.k_token_stride, v1 = a.c.v_token_stride, v8 = 8 * a.c.v_token_stride;
+                    const int64_t kr = S::ROWS * a.c.k_token_stride, vr = S::ROWS * a.c.v_token_stride;
+                    const uint32_t dst = ring + put, vdst = dst + 16 * D;
                     if (seen >= 16) {
 #pragma unroll
-                        for (int r = 0; r < 2; ++r)
+                        for (int r = 0; r < 16; r += S::ROWS) {
+                            cp_async16(dst + S::key_at(copy_row + r, copy_piece), kp);
+                            kp += kr;
+                        }
 #pragma unroll
-                            for (int h = 0; h < S::HALVES; ++h) cp_async16(dst + (r * S::HALVES + h) * 512, kp + r * k8 + h * 64);
-#pragma unroll
-                        for (int r = 0; r < 4; ++r)
-#pragma unroll
-                            for (int c = 0; c < S::VP; ++c) {
-                                const uint8_t *src = vp + (r & 1) * v1 + (r >> 1) * v8 + c * 128;
-                                if constexpr (S::VB == 16) cp_async16(vdst + (r * S::VP + c) * 512, src);
-                                else cp_async8(vdst + r * 256, src);
-                            }
+                        for (int r = 0; r < 16; r += S::ROWS) {
+                            cp_async16(vdst + S::value_at(copy_row + r, copy_piece), vp);
+                            vp += vr;
+                        }
                     } else {
 #pragma unroll
-                        for (int r = 0; r < 2; ++r)
-#pragma unroll
-                            for (int h = 0; h < S::HALVES; ++h)
-                                cp_async16_some(dst + (r * S::HALVES + h) * 512, kp + r * k8 + h * 64, g + 8 * r < seen ? 16 : 0);
-#pragma unroll
-                        for (int r = 0; r < 4; ++r)
-#pragma unroll
-                            for (int c = 0; c < S::VP; ++c) {
-                                const uint8_t *src = vp + (r & 1) * v1 + (r >> 1) * v8 + c * 128;
-                                const bool in = 2 * t + (r & 1) + (r >> 1) * 8 < seen;
-                                if constexpr (S::VB == 16) cp_async16_some(vdst + (r * S::VP + c) * 512, src, in ? 16 : 0);
-                                else cp_async8_some(vdst + r * 256, src, in ? 8 : 0);
-                            }
+                        for (int r = 0; r < 16; r += S::ROWS) {
+                            const int n = copy_row + r < seen ? 16 : 0;
+                            cp_async16_some(dst + S::key_at(copy_row + r, copy_piece), kp, n);
+                            cp_async16_some(vdst + S::value_at(copy_row + r, copy_piece), vp, n);
+                            kp += kr;
+                            vp += vr;
+                        }
                     }
                 }
                 ++issued;
@@ -359,6 +364,7 @@ __global__ void __launch_bounds__(kAttThreads, att_blocks(D, NT)) kv_attention_k
                     ks = ks_next, ok = ok_next, lv = log2f(vsafe), iv = 1.0f / vsafe;
                 }
                 cp_async_wait<S::STAGES - 2>();
+                __syncwarp();
                 const uint8_t *st0 = smem + warp * (S::STAGES * S::STAGE) + get;
                 float sc[2][NT][4];
 #pragma unroll
@@ -366,7 +372,8 @@ __global__ void __launch_bounds__(kAttThreads, att_blocks(D, NT)) kv_attention_k
                     const uint8_t *st = st0 + u * S::STAGE;
 #pragma unroll
                     for (int h = 0; h < S::HALVES; ++h) {
-                        const uint4 ka = *(const uint4 *)(st + h * 512 + lane * 16), kb = *(const uint4 *)(st + (S::HALVES + h) * 512 + lane * 16);
+                        const uint32_t at = S::key_at(g, 4 * h + t);
+                        const uint4 ka = *(const uint4 *)(st + at), kb = *(const uint4 *)(st + at + 8 * D);
                         const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
@@ -436,17 +443,18 @@ __global__ void __launch_bounds__(kAttThreads, att_blocks(D, NT)) kv_attention_k
                     }
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
-                    const uint8_t *sv = st0 + u * S::STAGE + 16 * D + lane * S::VB;
+                    const uint8_t *sv = st0 + u * S::STAGE + 16 * D;
 #pragma unroll
                     for (int c = 0; c < S::VP; ++c) {
                         uint32_t v[4][S::VB / 4];
 #pragma unroll
                         for (int r = 0; r < 4; ++r) {
+                            const int row = 2 * t + (r & 1) + (r >> 1) * 8;
                             if constexpr (S::VB == 16) {
-                                const uint4 x = *(const uint4 *)(sv + (r * S::VP + c) * 512);
+                                const uint4 x = *(const uint4 *)(sv + S::value_at(row, 8 * c + g));
                                 v[r][0] = code_word<INT8>(x.x), v[r][1] = code_word<INT8>(x.y), v[r][2] = code_word<INT8>(x.z), v[r][3] = code_word<INT8>(x.w);
                             } else {
-                                const uint2 x = *(const uint2 *)(sv + r * 256);
+                                const uint2 x = *(const uint2 *)(sv + S::value_at(row, g >> 1) + (g & 1) * 8);
                                 v[r][0] = code_word<INT8>(x.x), v[r][1] = code_word<INT8>(x.y);
                             }
                         }
@@ -461,6 +469,7 @@ __global__ void __launch_bounds__(kAttThreads, att_blocks(D, NT)) kv_attention_k
                     }
                 }
                 get = get == (S::STAGES - 2) * S::STAGE ? 0 : get + 2 * S::STAGE;
+                __syncwarp();
                 fetch();
                 fetch();
             }
@@ -553,15 +562,17 @@ constexpr int kJoinWarps = 16;
 
 template <int DT, int D, int NT>
 __global__ void __launch_bounds__(kJoinWarps * 32) kv_attention_join_kernel(const __grid_constant__ AttArgs a) {
-    constexpr int ROWS = NT * 8, E = D / 32, B = D == 256 ? 4 : 8;  // B: pieces in flight per warp
+    constexpr int ROWS = NT * 8, E = D / 32, B = D == 256 ? 2 : 4;  // B: pieces in flight per warp
     __shared__ float s_v[kJoinWarps][D], s_top[kJoinWarps], s_sum[kJoinWarps];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     grid_wait();
     const uint32_t pieces = (uint32_t)min((int64_t)__ldcg(a.pieces), a.slots);
-    for (uint32_t c = blockIdx.x; c < pieces; c += gridDim.x) {
-        const uint32_t last = __ldcg(&a.join[c].last);
-        if (last == 0) continue;
+    for (uint32_t c0 = blockIdx.x; c0 < pieces; c0 += 32 * gridDim.x)
+      for (uint32_t todo = __ballot_sync(0xffffffffu, c0 + lane * gridDim.x < pieces && __ldcg(&a.join[min(c0 + lane * gridDim.x, pieces - 1)].last) != 0); todo;
+           todo &= todo - 1) {
+        const uint32_t c = c0 + (__ffs(todo) - 1) * gridDim.x;
         const AttJoin it = a.join[c];
+        const uint32_t last = it.last;
         const int n = it.rows;
         // all warps on the rows: 16 / (n rounded up to a power of two) of them on each, every one with its share of the pieces
         const int log_rows = n <= 1 ? 0 : 32 - __clz(n - 1), log_warps = 4 - log_rows, r = warp & ((1 << log_rows) - 1);
@@ -671,7 +682,7 @@ static int att_launch(const AttArgs &a, cudaStream_t st) {
     rc = after_launch("kv_attention_kernel");
     // no request is longer than the shortest piece, and there is a block for each: nothing to join
     if (rc || (a.capacity <= kAttMinPiece * 16 && att_items(a.c, a.t, a.group, NT * 8) <= a.grid)) return rc;
-    return launch_dependent("kv_attention_join_kernel", kv_attention_join_kernel<DT, D, NT>, dim3((unsigned)a.grid), kJoinWarps * 32, 0, st, a);
+    return launch_dependent("kv_attention_join_kernel", kv_attention_join_kernel<DT, D, NT>, dim3((unsigned)sm_count()), kJoinWarps * 32, 0, st, a);
 }
 
 int kv_attention_launch(const ctb_kv_cache &c, const ctb_kv_batch &t, const void *q, int dtype, int64_t q_token_stride, int64_t q_head_stride, int q_heads,
