@@ -137,36 +137,33 @@ __global__ void __launch_bounds__(WARPS * 32) linear4_mma_kernel(const __grid_co
     };
     fetch_x(u0, min(u1, u0 + p.x_cols / 256));
 
-    // this lane's 16-byte pieces of every stage: rows g and g + 8, columns 32 t and 128 + 32 t of the 256
+    // this lane's 16-byte pieces of every stage (16 rows of 128 bytes): piece lane & 7 of rows lane >> 3, + 4, + 8, + 12, so that a
+    // warp instruction reads whole lines.  Pieces are permuted by the row's low bits: ldmatrix reads eight rows without a conflict.
     const int64_t row_a = row0 + g < a.rows ? row0 + g : a.rows - 1;  // rows behind the last one: read again, dropped at the end
     const int64_t row_b = row0 + g + 8 < a.rows ? row0 + g + 8 : a.rows - 1;
-    const uint8_t *src_a = (const uint8_t *)a.q + row_a * a.q_row_bytes + t * 16 + (int64_t)u0 * 128;
-    const uint8_t *src_b = (const uint8_t *)a.q + row_b * a.q_row_bytes + t * 16 + (int64_t)u0 * 128;
-    const uint32_t dst = ring + g * 64 + ((t ^ ((g >> 1) & 3)) << 4);  // the second row lies 512 bytes on, the second 128 columns 1024
+    const uint8_t *src[4];
+    uint32_t dst[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int r = (lane >> 3) + 4 * i;
+        src[i] = (const uint8_t *)a.q + (row0 + r < a.rows ? row0 + r : a.rows - 1) * a.q_row_bytes + (lane & 7) * 16 + (int64_t)u0 * 128;
+        dst[i] = ring + r * 128 + (((lane & 7) ^ (r & 7)) << 4);
+    }
     int left = u1 - u0;  // units that are not fetched yet
     const int last_cols = cols - (u1 - 1) * 256;  // columns of this share's last unit (more than there are: all 256)
     uint32_t put = 0;
     auto fetch = [&]() {
         if (left > 0) {
-            if (left > 1 || last_cols >= 256) {
-                cp_async16(dst + put, src_a);
-                cp_async16(dst + put + 512, src_b);
-                cp_async16(dst + put + 1024, src_a + 64);
-                cp_async16(dst + put + 1536, src_b + 64);
+            if (left > 1 || (lane & 7) * 32 < last_cols) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    cp_async16(dst[i] + put, src[i]);
+                    src[i] += 128;
+                }
             } else {
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    if (h * 128 + t * 32 < last_cols) {
-                        cp_async16(dst + put + h * 1024, src_a + h * 64);
-                        cp_async16(dst + put + h * 1024 + 512, src_b + h * 64);
-                    } else {
-                        st_shared16_zero(dst + put + h * 1024);
-                        st_shared16_zero(dst + put + h * 1024 + 512);
-                    }
-                }
+                for (int i = 0; i < 4; ++i) st_shared16_zero(dst[i] + put);
             }
-            src_a += 128;
-            src_b += 128;
             --left;
         }
         put = put == RING - 2048 ? 0 : put + 2048;
@@ -209,8 +206,10 @@ __global__ void __launch_bounds__(WARPS * 32) linear4_mma_kernel(const __grid_co
     };
     scales(2 * u0);
 
-    const uint32_t ldrow = (lane & 7) + ((lane >> 3) & 1) * 8, ldsw = (ldrow >> 1) & 3;
-    const uint32_t ld0 = ring + ldrow * 64 + (((lane >> 4) ^ ldsw) << 4), ld1 = ring + ldrow * 64 + (((2 + (lane >> 4)) ^ ldsw) << 4);
+    const uint32_t ldrow = (lane & 7) + ((lane >> 3) & 1) * 8;
+    uint32_t ld[4];  // 64 columns of 16 rows each
+#pragma unroll
+    for (int i = 0; i < 4; ++i) ld[i] = ring + ldrow * 128 + (((2 * i + (lane >> 4)) ^ (ldrow & 7)) << 4);
     float fin[NT][4];
 #pragma unroll
     for (int n = 0; n < NT; ++n)
@@ -246,10 +245,8 @@ __global__ void __launch_bounds__(WARPS * 32) linear4_mma_kernel(const __grid_co
             cp_async_wait<kLinStages - 1>();
             __syncwarp();
             uint32_t w[4][4];
-            ldmatrix4(w[0], ld0 + get);
-            ldmatrix4(w[1], ld1 + get);
-            ldmatrix4(w[2], ld0 + get + 1024);
-            ldmatrix4(w[3], ld1 + get + 1024);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) ldmatrix4(w[i], ld[i] + get);
             get = get == RING - 2048 ? 0 : get + 2048;
             __syncwarp();
             fetch();
