@@ -92,11 +92,8 @@ __device__ __forceinline__ uint32_t att_request_steps(const AttArgs &a, const Kv
     return n;
 }
 
-// Every warp walks the requests for itself, one per lane and 32 at a time; `first` is this lane's of the first 32.
 __device__ __forceinline__ KvSeq att_lane_seq(const AttArgs &a, const KvSeq &first, int base) {
-    const int b = base + (threadIdx.x & 31);
-    if (base == 0) return first;
-    return b < a.t.batch ? kv_seq(a.t, a.capacity, b) : KvSeq{0, 0, 0, 0};
+    return base == 0 ? first : kv_lane_seq(a.t, a.capacity, base);
 }
 
 // The whole line, over all requests and heads.  The host admits only calls whose line stays below 2^31 steps; row offsets
@@ -129,43 +126,12 @@ struct AttItem {
     uint32_t begin, steps, span;  // first step on the line; real steps; places on the line
 };
 
-__device__ __forceinline__ uint32_t warp_inclusive(uint32_t v) {
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t u = __shfl_up_sync(0xffffffffu, v, o);
-        if ((threadIdx.x & 31) >= o) v += u;
-    }
-    return v;
-}
-
-// What request weigh(seq) of every request sums up to `pos`: the request, its KvSeq and the sum in front of it, in all lanes.
-template <class F>
-__device__ __forceinline__ int att_locate(const AttArgs &a, const KvSeq &first, uint32_t pos, F weigh, KvSeq &s, uint32_t &begin) {
-    uint32_t run = 0;
-    for (int base = 0; base < a.t.batch; base += 32) {
-        const KvSeq q = att_lane_seq(a, first, base);
-        const uint32_t n = weigh(q), upto = run + warp_inclusive(n);
-        const uint32_t hit = __ballot_sync(0xffffffffu, pos < upto);
-        if (hit) {
-            const int src = __ffs(hit) - 1;
-            s.first_row = __shfl_sync(0xffffffffu, q.first_row, src);
-            s.rows = __shfl_sync(0xffffffffu, q.rows, src);
-            s.len = __shfl_sync(0xffffffffu, q.len, src);
-            s.start = __shfl_sync(0xffffffffu, q.start, src);
-            begin = __shfl_sync(0xffffffffu, upto - n, src);
-            return base + src;
-        }
-        run = __shfl_sync(0xffffffffu, upto, 31);
-    }
-    return -1;
-}
-
 // The item that holds position `pos` of the line.
 template <int NT>
 __device__ __forceinline__ AttItem att_find(const AttArgs &a, const AttCut &cut, const KvSeq &first, uint32_t pos) {
     AttItem it;
     const uint32_t heads = (uint32_t)a.c.heads;
-    it.b = att_locate(a, first, pos, [&](const KvSeq &q) { return att_request_steps<NT>(a, q, cut) * heads; }, it.s, it.begin);
+    it.b = kv_locate(a.t, a.capacity, first, pos, [&](const KvSeq &q) { return att_request_steps<NT>(a, q, cut) * heads; }, it.s, it.begin);
     const int tiles = it.b < 0 ? 0 : att_tiles<NT>(a, it.s);
     for (it.tile = 0; it.tile < tiles; ++it.tile) {
         it.steps = att_steps<NT>(a, it.s, it.tile);
@@ -220,7 +186,7 @@ __global__ void __launch_bounds__(kAttThreads, att_blocks(D, NT)) kv_attention_k
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ float s_m[kAttWarps][ROWS], s_l[kAttWarps][ROWS];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-    const KvSeq first = lane < a.t.batch ? kv_seq(a.t, a.capacity, lane) : KvSeq{0, 0, 0, 0};
+    const KvSeq first = kv_lane_seq(a.t, a.capacity, 0);
     grid_next();
     const AttCut cut = att_cut<NT>(a, first);
     if (blockIdx.x == 0 && threadIdx.x == 0) *a.pieces = (cut.total + cut.per - 1) / cut.per;

@@ -1,4 +1,7 @@
 // The 8-bit paged cache: quantized writes, and the attention over it for any head size and block size.
+#include <type_traits>
+
+#include "ctb_fastdiv.h"
 #include "ctb_kv_common.cuh"
 
 namespace ctb {
@@ -18,23 +21,45 @@ int kv_check(const ctb_kv_cache *c, const ctb_kv_batch *t, int32_t dtype) {
 }
 
 // ---------------------------------------------------------------- writing
-// One block of threads per (written cache block, head, keys or values): the absolute maximum over the rows that this
-// call writes there, the scale, the older codes again where the scale grew, the new codes.
+// What bounds it: two bytes read and one written per element, from and to HBM; for single tokens, the latency of a launch and
+// of four dependent loads (lengths, block number, rows and old scale, codes where the scale grew).
+//
+// A unit is one (written cache block, head, keys or values): the absolute maximum over the rows that the call writes
+// there, the scale, the older codes again where the scale grew, the new codes.  A unit is taken by a warp where the call
+// has about one row per request, else by a block of four; rows of 16-byte pieces stay in registers between the maximum and the
+// codes (up to PIECES of them per thread, which covers 64 x 128), what exceeds that is read again from the cache lines just read.
 //
 // A code is the grid value nearest to the exact quotient x / scale.  An fp32 quotient may round onto a tie that the
-// exact one is not on, so the quotient is rounded to odd (toward zero, last bit set when inexact): with 24 bits
-// against the grid's 4 (e4m3) or 8 (int8) the second rounding is then the only one.
-__device__ __forceinline__ float quotient_to_odd(float x, float s) {
-    const float q = __fdiv_rz(x, s);
-    const float r = fmaf(-q, s, x);
-    return r != 0.0f ? __uint_as_float(__float_as_uint(q) | 1u) : q;
+// exact one is not on, so the quotient is rounded to odd (where it is inexact, to the neighbour whose last bit is set): with 24 bits
+// against the grid's 4 (e4m3) or 8 (int8) the second rounding is then the only one.  `r` is 1 / s rounded; product, residual and
+// correction give the nearest quotient, and the sign of its own residual says on which side the exact one lies.  That matters only next
+// to a tie, whose low bits are zeros: x * r is within two units of the quotient, so a piece of eight takes the exact way only where
+// one of them comes within two units of such a number (one piece in ten thousand, and zeros).
+__device__ __forceinline__ float quotient_to_odd(float x, float s, float r) {
+    const float q0 = x * r, q = fmaf(fmaf(-q0, s, x), r, q0), e = fmaf(-q, s, x);
+    const int bits = __float_as_int(q);
+    // the residual has the quotient's sign where the exact magnitude is larger (the scale is positive)
+    const int step = (__float_as_int(e) ^ bits) < 0 ? -1 : 1;
+    return e != 0.0f && !(bits & 1) ? __int_as_float(bits + step) : q;
 }
 
 template <bool INT8>
-__device__ __forceinline__ uint8_t cache_code(float q) {
-    if (q != q) return 0;  // then the scale is an infinity or NaN: it alone marks the block, so that queries that do not see it stay clean
-    if constexpr (INT8) return (uint8_t)(int8_t)(int)fminf(fmaxf(rintf(q), -128.0f), 127.0f);
-    else return f32_to_e4m3(q);
+__device__ __forceinline__ bool near_a_tie(float q) {
+    return ((__float_as_uint(q) + 2u) & (INT8 ? 0x7fffu : 0x7ffffu)) <= 4u;
+}
+
+// two quotients -> two codes in the low bytes
+template <bool INT8>
+__device__ __forceinline__ uint32_t cache_codes2(float a, float b) {
+    if constexpr (INT8) {
+        // 1.5 * 2^23 + v has the integer nearest to v, ties to even, in its low byte
+        const float m = 12582912.0f;
+        return __byte_perm(__float_as_uint(fminf(fmaxf(a, -128.0f), 127.0f) + m), __float_as_uint(fminf(fmaxf(b, -128.0f), 127.0f) + m), 0x0040);
+    } else {
+        uint16_t r;
+        asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(b), "f"(a));
+        return r;
+    }
 }
 
 template <bool INT8>
@@ -43,81 +68,130 @@ __device__ __forceinline__ uint8_t cache_recode(uint8_t code, float before, floa
     const double v = (INT8 ? (double)(int8_t)code : (double)e4m3_to_f32(code)) * (double)before / (double)now;
     float f = __double2float_rz(v);
     if ((double)f != v) f = __uint_as_float(__float_as_uint(f) | 1u);
-    return cache_code<INT8>(f);
+    return (uint8_t)cache_codes2<INT8>(f, 0.0f);
 }
 
 constexpr int kAppendThreads = 128;
 
-template <int DT, bool INT8>
-__global__ void __launch_bounds__(kAppendThreads)
-kv_append_kernel(const ctb_kv_cache c, const ctb_kv_batch t, const void *k, const void *v, int64_t k_token_stride, int64_t k_head_stride,
-                 int64_t v_token_stride, int64_t v_head_stride) {
-    __shared__ int64_t tmp[kAppendThreads / 32];
-    __shared__ int s_request, s_block;
-    __shared__ uint32_t s_max[kAppendThreads / 32];
-    const int bs = c.block_size;
-    const int64_t capacity = t.table_width * bs;
-    // which request and which of its blocks: the written blocks of all requests are numbered in order
-    const int per = (t.batch + kAppendThreads - 1) / kAppendThreads;
-    const int b0 = threadIdx.x * per;
-    if (threadIdx.x == 0) s_request = -1;
-    auto written = [&](int b, int &first_block) { return kv_written_blocks(kv_seq(t, capacity, b), bs, first_block); };
-    int64_t mine = 0, total;
-    int fb;
-    for (int b = b0; b < b0 + per && b < t.batch; ++b) mine += written(b, fb);
-    int64_t at = block_exclusive<kAppendThreads>(mine, tmp, total);
-    const int64_t slot = blockIdx.x;
-    if (slot >= total) return;
-    if (slot >= at && slot < at + mine) {
-        for (int b = b0; b < b0 + per && b < t.batch; ++b) {
-            const int n = written(b, fb);
-            if (slot < at + n) {
-                s_request = b;
-                s_block = fb + (int)(slot - at);
-                break;
-            }
-            at += n;
-        }
-    }
-    __syncthreads();
-    const int b = s_request;
-    if (b < 0) return;
-    const KvSeq s = kv_seq(t, capacity, b);
-    const int page = t.block_table[b * t.table_stride + s_block];
-    if (page < 0 || page >= c.num_blocks) return;
-    const int p0 = max(max(s.start, 0), s_block * bs), p1 = min(s.len, (s_block + 1) * bs);
-    const int kept = p0 - s_block * bs;  // tokens of this request already in the block
-    const int head = blockIdx.y, dim = c.head_dim, n = (p1 - p0) * dim;
-    const bool values = blockIdx.z != 0;
-    const int64_t ts = values ? v_token_stride : k_token_stride;
-    const int64_t x0 = (int64_t)(s.first_row + (p0 - s.start)) * ts + (int64_t)head * (values ? v_head_stride : k_head_stride);
-    const void *x = values ? v : k;
-    uint8_t *codes = (uint8_t *)(values ? c.v : c.k) + (int64_t)page * (values ? c.v_block_stride : c.k_block_stride) +
-                     (int64_t)head * (values ? c.v_head_stride : c.k_head_stride);
-    const int64_t cs = values ? c.v_token_stride : c.k_token_stride;
-    float *scale = (values ? c.v_scale : c.k_scale) + (int64_t)page * c.heads + head;
+struct AppendArgs {
+    ctb_kv_cache c;
+    ctb_kv_batch t;
+    const void *x[2];                              // keys, values
+    int64_t token_stride[2], head_stride[2];
+    int64_t capacity;
+    FastDiv by_row;                                // pieces of a row
+    FastDiv by_groups;                             // groups of `per` units that the 2 * heads of a block make
+    uint32_t groups, per, total;                   // total: all groups that there may be
+};
 
-    uint32_t most = 0;  // bits of |x|: as integers they order like the numbers, with infinity and NaN on top
-    for (int i = threadIdx.x; i < n; i += kAppendThreads)
-        most = max(most, __float_as_uint(load_f32(x, DT, x0 + (int64_t)(i / dim) * ts + i % dim)) & 0x7fffffffu);
-    most = __reduce_max_sync(0xffffffffu, most);
-    if ((threadIdx.x & 31) == 0) s_max[threadIdx.x >> 5] = most;
-    const float before = kept > 0 ? *scale : 0.0f;
-    __syncthreads();
+// W: warps of a unit (1 or 4); V: elements that are loaded at once (8, or 1 for rows off the 16-byte grid)
+template <int DT, bool INT8, int W, int V>
+__global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const __grid_constant__ AppendArgs a) {
+    constexpr int T = W * 32, PIECES = 8;
+    __shared__ uint32_t s_max[kAppendThreads / 32];
+    const int lane = threadIdx.x & 31, i0 = threadIdx.x & (T - 1);
+    const uint32_t group = W == 4 ? blockIdx.x : blockIdx.x * 4 + (threadIdx.x >> 5);
+    if (group >= a.total) return;  // (with W == 4 for the whole block)
+    const uint32_t slot = fastdiv(group, a.by_groups);
+    const int first_unit = (int)((group - slot * a.groups) * a.per), bs = a.c.block_size, dim = a.c.head_dim;
+    // the written blocks of all requests are numbered in order
+    KvSeq s;
+    uint32_t begin;
+    int fb;
+    const int b = kv_locate(a.t, a.capacity, kv_lane_seq(a.t, a.capacity, 0), slot, [&](const KvSeq &q) { return (uint32_t)kv_written_blocks(q, bs, fb); }, s, begin);
+    if (b < 0) return;
+    kv_written_blocks(s, bs, fb);
+    const int block = fb + (int)(slot - begin);
+    const int page = a.t.block_table[b * a.t.table_stride + block];
+    if (page < 0 || page >= a.c.num_blocks) return;
+    const int p0 = max(max(s.start, 0), block * bs), p1 = min(s.len, (block + 1) * bs);
+    const int kept = p0 - block * bs;  // tokens of this request already in the block
+    const int row = dim / V, n = (p1 - p0) * row;
+    for (int u = first_unit; u < min(first_unit + (int)a.per, 2 * a.c.heads); ++u) {
+        const int values = u & 1, head = u >> 1;
+        const int64_t ts = a.token_stride[values], cs = values ? a.c.v_token_stride : a.c.k_token_stride;
+        const uint16_t *x = (const uint16_t *)a.x[values] + (int64_t)(s.first_row + (p0 - s.start)) * ts + (int64_t)head * a.head_stride[values];
+        uint8_t *codes = (uint8_t *)(values ? a.c.v : a.c.k) + (int64_t)page * (values ? a.c.v_block_stride : a.c.k_block_stride) +
+                         (int64_t)head * (values ? a.c.v_head_stride : a.c.k_head_stride);
+        float *scale = (values ? a.c.v_scale : a.c.k_scale) + (int64_t)page * a.c.heads + head;
+        const float before = kept > 0 ? *scale : 0.0f;
+
+        // pieces i0, i0 + T, ... of the rows in order
+        auto load = [&](int i) {
+            const int tk = (int)fastdiv((uint32_t)i, a.by_row), d = (i - tk * row) * V;
+            if constexpr (V == 8) return __ldg((const uint4 *)(x + tk * ts + d));
+            else return make_uint4(x[tk * ts + d], 0, 0, 0);
+        };
+        uint4 held[PIECES];
+        uint32_t most = 0;  // bits of |x|, two at a time: as integers they order like the numbers, with infinity and NaN on top
+        auto weigh = [&](const uint4 &v) {
+            most = __vmaxu2(most, __vmaxu2(__vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu), __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu)));
+        };
 #pragma unroll
-    for (int w = 0; w < kAppendThreads / 32; ++w) most = max(most, s_max[w]);
-    float now = __fdiv_rn(__uint_as_float(most), INT8 ? 127.5f : 448.0f);
-    now = now != now ? now : fmaxf(now, 1.1920928955078125e-07f);
-    if (kept > 0) now = (before > now || before != before) ? before : now;
-    if (threadIdx.x == 0) *scale = now;
-    if (kept > 0 && now > before)
-        for (int i = threadIdx.x; i < kept * dim; i += kAppendThreads) {
-            uint8_t *p = codes + (int64_t)(i / dim) * cs + i % dim;
-            *p = cache_recode<INT8>(*p, before, now);
+        for (int k = 0; k < PIECES; ++k) held[k] = i0 + k * T < n ? load(i0 + k * T) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int k = 0; k < PIECES; ++k) weigh(held[k]);
+        for (int i = i0 + PIECES * T; i < n; i += T) weigh(load(i));
+        most = __reduce_max_sync(0xffffffffu, max(most & 0xffffu, most >> 16));
+        if constexpr (W > 1) {
+            __syncthreads();  // the unit before has been read
+            if (lane == 0) s_max[threadIdx.x >> 5] = most;
+            __syncthreads();
+#pragma unroll
+            for (int w = 0; w < W; ++w) most = max(most, s_max[w]);
         }
-    for (int i = threadIdx.x; i < n; i += kAppendThreads)
-        codes[(int64_t)(kept + i / dim) * cs + i % dim] =
-            cache_code<INT8>(quotient_to_odd(load_f32(x, DT, x0 + (int64_t)(i / dim) * ts + i % dim), now));
+        const float top = DT == CTB_BF16 ? bf16_bits_to_f32(most) : __half2float(__ushort_as_half((unsigned short)most));
+        float now = __fdiv_rn(top, INT8 ? 127.5f : 448.0f);
+        now = now != now ? now : fmaxf(now, 1.1920928955078125e-07f);
+        if (kept > 0) now = (before > now || before != before) ? before : now;
+        __syncwarp();
+        if (i0 == 0) *scale = now;
+        // an infinity or NaN marks its block by the scale alone (codes of zero), so that queries that do not see it stay clean
+        const bool finite = now - now == 0.0f;
+        if (kept > 0 && now > before)
+            for (int i = i0; i < kept * row; i += T) {
+                uint8_t *p = codes + (int64_t)(i / row) * cs + (i % row) * V;
+                if constexpr (V == 8) {
+                    uint2 w = *(const uint2 *)p;
+                    uint8_t(&c)[8] = reinterpret_cast<uint8_t(&)[8]>(w);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) c[e] = finite ? cache_recode<INT8>(c[e], before, now) : 0;
+                    *(uint2 *)p = w;
+                } else {
+                    *p = finite ? cache_recode<INT8>(*p, before, now) : 0;
+                }
+            }
+        const float r = __frcp_rn(now);
+        auto half = [](uint32_t h) { return DT == CTB_BF16 ? bf16_bits_to_f32(h) : __half2float(__ushort_as_half((unsigned short)h)); };
+        auto store = [&](int i, const uint4 &v) {
+            const int tk = (int)fastdiv((uint32_t)i, a.by_row), d = (i - tk * row) * V;
+            uint8_t *p = codes + (int64_t)(kept + tk) * cs + d;
+            const uint32_t h[4] = {v.x, v.y, v.z, v.w};
+            float q[8];
+            bool near = false;
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                q[e] = half(e & 1 ? h[e >> 1] >> 16 : h[e >> 1] & 0xffffu) * r;
+                near |= near_a_tie<INT8>(q[e]);
+            }
+            if (near) {
+#pragma unroll
+                for (int e = 0; e < V; ++e) q[e] = quotient_to_odd(half(e & 1 ? h[e >> 1] >> 16 : h[e >> 1] & 0xffffu), now, r);
+            }
+            if constexpr (V == 8) {
+                uint2 w = make_uint2(__byte_perm(cache_codes2<INT8>(q[0], q[1]), cache_codes2<INT8>(q[2], q[3]), 0x5410),
+                                     __byte_perm(cache_codes2<INT8>(q[4], q[5]), cache_codes2<INT8>(q[6], q[7]), 0x5410));
+            if (!finite) w = make_uint2(0, 0);
+                *(uint2 *)p = w;
+            } else {
+                *p = finite ? (uint8_t)cache_codes2<INT8>(q[0], 0.0f) : 0;
+            }
+        };
+#pragma unroll
+        for (int k = 0; k < PIECES; ++k)
+            if (i0 + k * T < n) store(i0 + k * T, held[k]);
+        for (int i = i0 + PIECES * T; i < n; i += T) store(i, load(i));
+    }
 }
 
 // ---------------------------------------------------------------- attention, any head size
@@ -213,19 +287,41 @@ extern "C" int ctb_kv_cache_append(const ctb_kv_cache *c, const ctb_kv_batch *t,
     if (rc) return rc;
     if (t->batch == 0 || t->tokens == 0 || c->num_blocks == 0) return CTB_OK;
     if (!k || !v) return fail(CTB_EINVAL_NULL, "null keys or values");
-    if (c->heads > 65535) return fail(CTB_EUNSUPPORTED, "too many heads");
-    const int64_t slots = kv_most_written(t->tokens, t->batch, c->block_size);
-    const dim3 grid((unsigned)slots, (unsigned)c->heads, 2);
+    const int64_t units = kv_most_written(t->tokens, t->batch, c->block_size) * 2 * c->heads;
+    if (units > INT32_MAX - 4) return fail(CTB_EUNSUPPORTED, "too many tokens and heads for one call");
+    AppendArgs a;
+    a.c = *c;
+    a.t = *t;
+    a.x[0] = k, a.x[1] = v;
+    a.token_stride[0] = k_token_stride, a.token_stride[1] = v_token_stride;
+    a.head_stride[0] = k_head_stride, a.head_stride[1] = v_head_stride;
+    a.capacity = t->table_width * c->block_size;
     const cudaStream_t st = as_stream(stream);
-#define CTB_APPEND(DT, I8) kv_append_kernel<DT, I8><<<grid, kAppendThreads, 0, st>>>(*c, *t, k, v, k_token_stride, k_head_stride, v_token_stride, v_head_stride)
-    if (dtype == CTB_BF16) {
-        if (c->dtype == CTB_I8) CTB_APPEND(CTB_BF16, true);
-        else CTB_APPEND(CTB_BF16, false);
-    } else {
-        if (c->dtype == CTB_I8) CTB_APPEND(CTB_F16, true);
-        else CTB_APPEND(CTB_F16, false);
-    }
-#undef CTB_APPEND
+    const bool wide = c->head_dim % 8 == 0 && aligned16(k) && aligned16(v) && (k_token_stride | k_head_stride | v_token_stride | v_head_stride) % 8 == 0 &&
+                      (((uintptr_t)c->k | (uintptr_t)c->v) & 7) == 0 &&
+                      (c->k_block_stride | c->k_head_stride | c->k_token_stride | c->v_block_stride | c->v_head_stride | c->v_token_stride) % 8 == 0;
+    // a warp per unit where its rows fit the warp's registers: about one row per request, or small blocks; else a block of four
+    const bool single = t->tokens <= 2 * (int64_t)t->batch || (int64_t)c->block_size * c->head_dim <= 2048;
+    // Several units of a cache block in turn, once there are enough of them to fill the GPU: the search for the request is made
+    // once for all.
+    a.per = units >= 16 * (int64_t)sm_count() * (single ? 4 : 1) ? 4 : 1;
+    a.by_row = make_fastdiv((uint32_t)(wide ? c->head_dim / 8 : c->head_dim));
+    a.groups = (uint32_t)cdiv(2 * c->heads, a.per);
+    a.by_groups = make_fastdiv(a.groups);
+    a.total = (uint32_t)(kv_most_written(t->tokens, t->batch, c->block_size) * a.groups);
+    auto go = [&](auto dt, auto i8) {
+        constexpr int DT = decltype(dt)::value;
+        constexpr bool I8 = decltype(i8)::value;
+        const unsigned blocks = (unsigned)(single ? cdiv(a.total, 4) : a.total);
+        if (wide && single) kv_append_kernel<DT, I8, 1, 8><<<blocks, kAppendThreads, 0, st>>>(a);
+        else if (wide) kv_append_kernel<DT, I8, 4, 8><<<blocks, kAppendThreads, 0, st>>>(a);
+        else if (single) kv_append_kernel<DT, I8, 1, 1><<<blocks, kAppendThreads, 0, st>>>(a);
+        else kv_append_kernel<DT, I8, 4, 1><<<blocks, kAppendThreads, 0, st>>>(a);
+    };
+    using B = std::integral_constant<int, CTB_BF16>;
+    using H = std::integral_constant<int, CTB_F16>;
+    if (dtype == CTB_BF16) c->dtype == CTB_I8 ? go(B{}, std::true_type{}) : go(B{}, std::false_type{});
+    else c->dtype == CTB_I8 ? go(H{}, std::true_type{}) : go(H{}, std::false_type{});
     return after_launch("kv_append_kernel");
 }
 

@@ -10,27 +10,42 @@ __device__ __forceinline__ KvSeq kv_seq(const ctb_kv_batch &t, int64_t capacity,
     return kv_seq(t.query_start[b], t.query_start[b + 1], t.seq_lens[b], t.tokens, capacity);
 }
 
-// Exclusive scan of `mine` over a block of THREADS threads; `total` gets the sum.  `tmp`: THREADS / 32 shared words.
-template <int THREADS>
-__device__ __forceinline__ int64_t block_exclusive(int64_t mine, int64_t *tmp, int64_t &total) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int64_t v = mine;
+__device__ __forceinline__ uint32_t warp_inclusive(uint32_t v) {
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const int64_t u = __shfl_up_sync(0xffffffffu, v, o);
-        if (lane >= o) v += u;
+        const uint32_t u = __shfl_up_sync(0xffffffffu, v, o);
+        if ((threadIdx.x & 31) >= o) v += u;
     }
-    if (lane == 31) tmp[warp] = v;
-    __syncthreads();
-    int64_t before = 0;
-    total = 0;
-#pragma unroll
-    for (int w = 0; w < THREADS / 32; ++w) {
-        if (w < warp) before += tmp[w];
-        total += tmp[w];
+    return v;
+}
+
+// Every warp walks the requests for itself, one per lane and 32 at a time; `first` is this lane's of the first 32.
+__device__ __forceinline__ KvSeq kv_lane_seq(const ctb_kv_batch &t, int64_t capacity, int base) {
+    const int b = base + (threadIdx.x & 31);
+    return b < t.batch ? kv_seq(t, capacity, b) : KvSeq{0, 0, 0, 0};
+}
+
+// The request that `pos` falls into when weigh(request) numbers are counted off for each in turn, -1 behind the last; its KvSeq and the
+// number it begins at, in all lanes.  The numbers of all requests stay below 2^32.
+template <class F>
+__device__ __forceinline__ int kv_locate(const ctb_kv_batch &t, int64_t capacity, const KvSeq &first, uint32_t pos, F weigh, KvSeq &s, uint32_t &begin) {
+    uint32_t run = 0;
+    for (int base = 0; base < t.batch; base += 32) {
+        const KvSeq q = base == 0 ? first : kv_lane_seq(t, capacity, base);
+        const uint32_t n = weigh(q), upto = run + warp_inclusive(n);
+        const uint32_t hit = __ballot_sync(0xffffffffu, pos < upto);
+        if (hit) {
+            const int src = __ffs(hit) - 1;
+            s.first_row = __shfl_sync(0xffffffffu, q.first_row, src);
+            s.rows = __shfl_sync(0xffffffffu, q.rows, src);
+            s.len = __shfl_sync(0xffffffffu, q.len, src);
+            s.start = __shfl_sync(0xffffffffu, q.start, src);
+            begin = __shfl_sync(0xffffffffu, upto - n, src);
+            return base + src;
+        }
+        run = __shfl_sync(0xffffffffu, upto, 31);
     }
-    __syncthreads();
-    return before + v - mine;
+    return -1;
 }
 
 // host: what every entry point refuses
