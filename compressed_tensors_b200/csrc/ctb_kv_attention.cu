@@ -286,13 +286,13 @@ __global__ void __launch_bounds__(kAttThreads, att_blocks(D, NT)) kv_attention_k
             int end[NT][2];   // positions that rows 2t, 2t + 1 see
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-                uint32_t most = 0;  // as integers the absolute values order like the numbers, with infinity and NaN on top
+                uint32_t most = 0;
 #pragma unroll
                 for (int k = 0; k < D / 32; ++k)
-                    most = __vmaxu2(most, __vmaxu2(__vmaxu2(qraw[n][k].x & 0x7fff7fffu, qraw[n][k].y & 0x7fff7fffu),
-                                                   __vmaxu2(qraw[n][k].z & 0x7fff7fffu, qraw[n][k].w & 0x7fff7fffu)));
-                most = __vmaxu2(most, __shfl_xor_sync(0xffffffffu, most, 1));
-                most = __vmaxu2(most, __shfl_xor_sync(0xffffffffu, most, 2));
+                    most = max2_nan<DT>(most, max2_nan<DT>(max2_nan<DT>(qraw[n][k].x & 0x7fff7fffu, qraw[n][k].y & 0x7fff7fffu),
+                                                           max2_nan<DT>(qraw[n][k].z & 0x7fff7fffu, qraw[n][k].w & 0x7fff7fffu)));
+                most = max2_nan<DT>(most, __shfl_xor_sync(0xffffffffu, most, 1));
+                most = max2_nan<DT>(most, __shfl_xor_sync(0xffffffffu, most, 2));
                 const float top = half_f32<DT>(max(most & 0xffffu, most >> 16));
                 const int e = max((int)(__float_as_uint(top) >> 23), 8);
                 const float up = __uint_as_float((uint32_t)(261 - e) << 23);  // the largest element comes to [128, 256)

@@ -3,6 +3,7 @@
 
 #include "ctb_fastdiv.h"
 #include "ctb_kv_common.cuh"
+#include "ctb_mma.cuh"
 
 namespace ctb {
 
@@ -32,20 +33,19 @@ int kv_check(const ctb_kv_cache *c, const ctb_kv_batch *t, int32_t dtype) {
 // A code is the grid value nearest to the exact quotient x / scale.  An fp32 quotient may round onto a tie that the
 // exact one is not on, so the quotient is rounded to odd (where it is inexact, to the neighbour whose last bit is set): with 24 bits
 // against the grid's 4 (e4m3) or 8 (int8) the second rounding is then the only one.  `r` is 1 / s rounded; product, residual and
-// correction give the nearest quotient, and the sign of its own residual says on which side the exact one lies.  That matters only next
-// to a tie, whose low bits are zeros: x * r is within two units of the quotient, so a piece of eight takes the exact way only where
-// one of them comes within two units of such a number (one piece in ten thousand, and zeros).
+// correction give the nearest quotient, and the sign of its own residual says on which side the exact one lies.
+//
+// Where the scale was just made from the rows themselves, s = round(m / h) with m their largest magnitude and h = 448 or 127.5, one
+// product replaces that.  x and m have at most 11 significant bits, a tie of the grid at most 9, h at most 8: x h and m tie are
+// integers of at most 20 bits times powers of two, equal or 2^-20 apart.  So a quotient is 2^-20 away from every tie, or it would be on
+// one if s were exactly m / h: then it lies on the side that the rounding of s puts all of them on, and a factor of 1 -+ 2^-22, which
+// the roundings of the quotient and the product (2^-24 each) cannot undo, moves it there.  Where m / h needs no rounding the factor is 1.
 __device__ __forceinline__ float quotient_to_odd(float x, float s, float r) {
     const float q0 = x * r, q = fmaf(fmaf(-q0, s, x), r, q0), e = fmaf(-q, s, x);
     const int bits = __float_as_int(q);
     // the residual has the quotient's sign where the exact magnitude is larger (the scale is positive)
     const int step = (__float_as_int(e) ^ bits) < 0 ? -1 : 1;
     return e != 0.0f && !(bits & 1) ? __int_as_float(bits + step) : q;
-}
-
-template <bool INT8>
-__device__ __forceinline__ bool near_a_tie(float q) {
-    return ((__float_as_uint(q) + 2u) & (INT8 ? 0x7fffu : 0x7ffffu)) <= 4u;
 }
 
 // two quotients -> two codes in the low bytes
@@ -86,7 +86,7 @@ struct AppendArgs {
 
 // W: warps of a unit (1 or 4); V: elements that are loaded at once (8, or 1 for rows off the 16-byte grid)
 template <int DT, bool INT8, int W, int V>
-__global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const __grid_constant__ AppendArgs a) {
+__global__ void __launch_bounds__(kAppendThreads, 6) kv_append_kernel(const __grid_constant__ AppendArgs a) {
     constexpr int T = W * 32, PIECES = 8;
     __shared__ uint32_t s_max[kAppendThreads / 32];
     const int lane = threadIdx.x & 31, i0 = threadIdx.x & (T - 1);
@@ -123,9 +123,9 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const __grid_
             else return make_uint4(x[tk * ts + d], 0, 0, 0);
         };
         uint4 held[PIECES];
-        uint32_t most = 0;  // bits of |x|, two at a time: as integers they order like the numbers, with infinity and NaN on top
+        uint32_t most = 0;  // |x|, two at a time
         auto weigh = [&](const uint4 &v) {
-            most = __vmaxu2(most, __vmaxu2(__vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu), __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu)));
+            most = max2_nan<DT>(most, max2_nan<DT>(max2_nan<DT>(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu), max2_nan<DT>(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu)));
         };
 #pragma unroll
         for (int k = 0; k < PIECES; ++k) held[k] = i0 + k * T < n ? load(i0 + k * T) : make_uint4(0, 0, 0, 0);
@@ -141,8 +141,12 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const __grid_
             for (int w = 0; w < W; ++w) most = max(most, s_max[w]);
         }
         const float top = DT == CTB_BF16 ? bf16_bits_to_f32(most) : __half2float(__ushort_as_half((unsigned short)most));
-        float now = __fdiv_rn(top, INT8 ? 127.5f : 448.0f);
-        now = now != now ? now : fmaxf(now, 1.1920928955078125e-07f);
+        constexpr float half_range = INT8 ? 127.5f : 448.0f;
+        float now = __fdiv_rn(top, half_range);
+        const float off = fmaf(now, half_range, -top);  // how the rounding went
+        float side = off > 0.0f ? 1.0f - 0x1p-22f : off < 0.0f ? 1.0f + 0x1p-22f : 1.0f;
+        if (now < 1.1920928955078125e-07f) now = 1.1920928955078125e-07f, side = 1.0f;  // a power of two: quotients are exact
+        const bool fresh = kept == 0 || now > before;
         if (kept > 0) now = (before > now || before != before) ? before : now;
         __syncwarp();
         if (i0 == 0) *scale = now;
@@ -168,20 +172,20 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const __grid_
             uint8_t *p = codes + (int64_t)(kept + tk) * cs + d;
             const uint32_t h[4] = {v.x, v.y, v.z, v.w};
             float q[8];
-            bool near = false;
 #pragma unroll
             for (int e = 0; e < V; ++e) {
-                q[e] = half(e & 1 ? h[e >> 1] >> 16 : h[e >> 1] & 0xffffu) * r;
-                near |= near_a_tie<INT8>(q[e]);
-            }
-            if (near) {
-#pragma unroll
-                for (int e = 0; e < V; ++e) q[e] = quotient_to_odd(half(e & 1 ? h[e >> 1] >> 16 : h[e >> 1] & 0xffffu), now, r);
+                const float f = half(e & 1 ? h[e >> 1] >> 16 : h[e >> 1] & 0xffffu);
+                if (fresh) {
+                    const float q0 = f * r;
+                    q[e] = fmaf(fmaf(-q0, now, f), r, q0) * side;
+                } else {
+                    q[e] = quotient_to_odd(f, now, r);
+                }
             }
             if constexpr (V == 8) {
                 uint2 w = make_uint2(__byte_perm(cache_codes2<INT8>(q[0], q[1]), cache_codes2<INT8>(q[2], q[3]), 0x5410),
                                      __byte_perm(cache_codes2<INT8>(q[4], q[5]), cache_codes2<INT8>(q[6], q[7]), 0x5410));
-            if (!finite) w = make_uint2(0, 0);
+                if (!finite) w = make_uint2(0, 0);
                 *(uint2 *)p = w;
             } else {
                 *p = finite ? (uint8_t)cache_codes2<INT8>(q[0], 0.0f) : 0;

@@ -135,6 +135,14 @@ __device__ __forceinline__ uint32_t sub2(uint32_t a, uint32_t b) {
     else asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
     return r;
 }
+// the larger of each half, NaN where one of them is NaN; for non-negative numbers the result also orders as an integer
+template <int DT>
+__device__ __forceinline__ uint32_t max2_nan(uint32_t a, uint32_t b) {
+    uint32_t r;
+    if constexpr (DT == CTB_BF16) asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    else asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
 template <int DT>
 __device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b) {
     uint32_t r;
