@@ -2,6 +2,7 @@
 current CUDA stream, turn status codes into exceptions.  Every function launches hand-written
 sm_100a kernels; none has a CPU path."""
 import ctypes
+import struct
 from typing import Optional, Tuple
 
 import torch
@@ -578,8 +579,15 @@ def unpack_dequantize_int4_batch(table, device=None):
 
 
 # ---------------------------------------------------------------- serving a compressed model
+# A decoding step makes several of these calls for a few microseconds of GPU work each, so a valid call is recognised by one
+# condition and its descriptors are packed at once; what is wrong with another is found out afterwards.
 
 _HALF = (torch.bfloat16, torch.float16)
+_CODES = (torch.int8, torch.float8_e4m3fn)
+_SCALES = (torch.bfloat16, torch.float16, torch.float32, torch.float8_e4m3fn)
+_QDESC = struct.Struct("@5q8i").pack          # ctb_qdesc
+_KV_CACHE = struct.Struct("@4Q7q4i").pack     # ctb_kv_cache
+_KV_BATCH = struct.Struct("@3Q3q2i").pack     # ctb_kv_batch
 
 
 def _same_device(first, *rest):
@@ -589,26 +597,19 @@ def _same_device(first, *rest):
             raise ValueError(f"all tensors of a call must be on one device, got {first.device} and {t.device}")
 
 
-def _call(device, fn, *args):
+def _call(device: int, fn, *args):
     """`fn(*args, stream)` with `device` current, on its current stream."""
-    stream = torch.cuda.current_stream(device).cuda_stream
-    if device.index == torch.cuda.current_device():
-        check(fn(*args, stream))
+    stream = torch._C._cuda_getCurrentRawStream(device)
+    if device == torch._C._cuda_getDevice():
+        status = fn(*args, stream)
     else:
         with torch.cuda.device(device):
-            check(fn(*args, stream))
+            status = fn(*args, stream)
+    if status:
+        check(status)
 
 
-def _dp(t):
-    return None if t is None else t.data_ptr()
-
-
-def dequantize_linear(x, q, scale, zp=None, *, qtype, bits=4, col_group, scale_row_stride, codec="pack32", global_scale=None, bias=None):
-    """x @ dequantize(q, scale, zp).T + bias without the dense weight in memory, for few tokens (every 32 read `q` again).
-
-    x [..., cols] bf16 / f16; q as `dequantize` takes it: int32 words [rows, ceil(cols / 8)] (codec "pack32", qtype QINT) or
-    uint8 pairs [rows, cols / 2] (codec "fp4x2", qtype QFLOAT); scale, zp (int8) and global_scale as there; bias [rows] of
-    x's dtype.  The dequantized weight is not rounded: products and sums are fp32, the result is rounded once."""
+def _refuse_linear(x, q, scale, zp, qtype, bits, col_group, scale_row_stride, codec, global_scale, bias):
     if codec not in ("pack32", "fp4x2"):
         raise NotImplementedError(f"the product takes packed codes (pack32, fp4x2), got {codec!r}")
     if bits != 4 or qtype != (QINT if codec == "pack32" else QFLOAT):
@@ -622,7 +623,7 @@ def dequantize_linear(x, q, scale, zp=None, *, qtype, bits=4, col_group, scale_r
     rows, cols = q.shape[0], x.shape[-1]
     if q.shape[1] != ((cols + 7) // 8 if codec == "pack32" else cols // 2) or (codec == "fp4x2" and cols % 2):
         raise ValueError(f"packed weight of shape {tuple(q.shape)} does not hold {cols} columns")
-    if scale.dtype not in (*_HALF, torch.float32, torch.float8_e4m3fn):
+    if scale.dtype not in _SCALES:
         raise TypeError(f"unsupported scale dtype {scale.dtype}")
     if rows and cols:
         if col_group < 1 or cols % col_group:
@@ -646,31 +647,41 @@ def dequantize_linear(x, q, scale, zp=None, *, qtype, bits=4, col_group, scale_r
     if bias is not None and (bias.dtype is not x.dtype or tuple(bias.shape) != (rows,)):
         raise ValueError(f"bias must be a {x.dtype} tensor of shape ({rows},)")
     _same_device(x, q, scale, zp, bias)
-    x, q, scale, zp, bias = _c(x), _c(q), _c(scale), _c(zp), _c(bias)
-    out = torch.empty(x.shape[:-1] + (rows,), dtype=x.dtype, device=x.device)
-    d = QDesc(rows, cols, col_group, 1, scale_row_stride, qtype, bits, DT[x.dtype], DT[scale.dtype], L.I8, 0, _CODEC[codec], 0)
+
+
+def dequantize_linear(x, q, scale, zp=None, *, qtype, bits=4, col_group, scale_row_stride, codec="pack32", global_scale=None, bias=None):
+    """x @ dequantize(q, scale, zp).T + bias without the dense weight in memory, for few tokens (every 32 read `q` again).
+
+    x [..., cols] bf16 / f16; q as `dequantize` takes it: int32 words [rows, ceil(cols / 8)] (codec "pack32", qtype QINT) or
+    uint8 pairs [rows, cols / 2] (codec "fp4x2", qtype QFLOAT); scale, zp (int8) and global_scale as there; bias [rows] of
+    x's dtype.  The dequantized weight is not rounded: products and sums are fp32, the result is rounded once.  Rows of whole
+    16-byte pieces (cols a multiple of 32) with scale groups of a multiple of 32 columns (16 with e4m3 scales for fp4x2) run on
+    the tensor cores; other sizes run one code at a time."""
+    shape, device = x.shape, x.get_device()
+    rows, cols = (q.shape[0], shape[-1]) if len(shape) and q.dim() == 2 else (0, 0)
+    if not (rows and cols and bits == 4 and x.dtype in _HALF and col_group > 0 and cols % col_group == 0 and scale_row_stride >= 0
+            and (codec == "pack32" and qtype == QINT and q.dtype is torch.int32 and q.shape[1] == (cols + 7) // 8 and global_scale is None
+                 or codec == "fp4x2" and qtype == QFLOAT and q.dtype is torch.uint8 and q.shape[1] * 2 == cols and zp is None
+                 and (global_scale is None or global_scale.numel() == 1))
+            and scale.dtype in _SCALES and scale.numel() >= (rows - 1) * scale_row_stride + cols // col_group and zp is None and bias is None
+            and device >= 0 and q.get_device() == device and scale.get_device() == device):
+        _refuse_linear(x, q, scale, zp, qtype, bits, col_group, scale_row_stride, codec, global_scale, bias)
+        zp, bias = _c(zp), _c(bias)
+    x, q, scale = x.contiguous(), q.contiguous(), scale.contiguous()
+    out = torch.empty(shape[:-1] + (rows,), dtype=x.dtype, device=x.device)
+    d = _QDESC(rows, cols, col_group, 1, scale_row_stride, qtype, bits, DT[x.dtype], DT[scale.dtype], L.I8, 0, _CODEC[codec], 0)
     gs = _gs(global_scale, x)
     tokens = x.numel() // cols if cols else out.numel() // max(rows, 1)
-    _call(x.device, lib().ctb_dequantize_linear, ctypes.addressof(d), x.data_ptr(), tokens, q.data_ptr(), scale.data_ptr(), _dp(zp),
-          _dp(gs), _dp(bias), out.data_ptr())
+    _call(device, lib().ctb_dequantize_linear, d, x.data_ptr(), tokens, q.data_ptr(), scale.data_ptr(),
+          None if zp is None else zp.data_ptr(), None if gs is None else gs.data_ptr(), None if bias is None else bias.data_ptr(), out.data_ptr())
     return out
 
 
-def _rows_of_heads(t, name, heads, dim):
-    """[tokens, heads, dim] with contiguous heads and 16-byte steps: as it is where it has them (a slice of a fused
-    projection does), else a copy."""
-    if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != dim:
-        raise ValueError(f"{name} must be [tokens, {heads}, {dim}], got {tuple(t.shape)}")
-    if dim > 1 and t.stride(2) != 1:
-        return t.contiguous()
-    return t
-
-
-def _kv_structs(x, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, query_start):
-    """Checks what append and attention share and builds their descriptors; returns them with what has to stay alive."""
+def _refuse_kv(x, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, query_start):
+    """Says what is wrong with a call of append or attention; int64 tables and lengths are the one thing that is not."""
     if k_cache.dim() != 4 or v_cache.shape != k_cache.shape:
         raise ValueError(f"k_cache and v_cache must be [num_blocks, heads, block_size, head_dim], got {tuple(k_cache.shape)} and {tuple(v_cache.shape)}")
-    if k_cache.dtype not in (torch.int8, torch.float8_e4m3fn) or v_cache.dtype is not k_cache.dtype:
+    if k_cache.dtype not in _CODES or v_cache.dtype is not k_cache.dtype:
         raise TypeError(f"the cache holds int8 or float8_e4m3fn codes, got {k_cache.dtype} and {v_cache.dtype}")
     if x.dtype not in _HALF:
         raise TypeError(f"queries, keys and values must be bfloat16 or float16, got {x.dtype}")
@@ -692,16 +703,40 @@ def _kv_structs(x, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, qu
     if block_table.shape[0] != batch or query_start.shape[0] != batch + 1:
         raise ValueError(f"{batch} lengths need a block table of {batch} rows and {batch + 1} row offsets, got {block_table.shape[0]} and {query_start.shape[0]}")
     _same_device(x, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, query_start)
-    block_table, seq_lens, query_start = (t if t.dtype is torch.int32 else t.to(torch.int32) for t in (block_table, seq_lens, query_start))
-    if block_table.stride(1) != 1 and block_table.shape[1] > 1:
+
+
+def _kv_structs(x, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, query_start):
+    """The packed descriptors of a call, and what has to stay alive until it is made."""
+    shape, dt, batch = k_cache.shape, k_cache.dtype, seq_lens.shape[0]
+    i32, device = torch.int32, x.get_device()
+    if not (len(shape) == 4 and v_cache.shape == shape and dt in _CODES and v_cache.dtype is dt and x.dtype in _HALF and shape[1] > 0 and shape[2] > 0
+            and 0 < shape[3] <= 256 and k_cache.stride(3) == 1 and v_cache.stride(3) == 1
+            and k_scale.dtype is torch.float32 and v_scale.dtype is torch.float32 and k_scale.shape == shape[:2] and v_scale.shape == shape[:2]
+            and k_scale.is_contiguous() and v_scale.is_contiguous()
+            and block_table.dtype is i32 and seq_lens.dtype is i32 and query_start.dtype is i32 and seq_lens.dim() == 1 and query_start.dim() == 1
+            and block_table.dim() == 2 and block_table.shape[0] == batch and query_start.shape[0] == batch + 1
+            and device >= 0 and k_cache.get_device() == device and v_cache.get_device() == device and k_scale.get_device() == device
+            and v_scale.get_device() == device and block_table.get_device() == device and seq_lens.get_device() == device
+            and query_start.get_device() == device):
+        _refuse_kv(x, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, query_start)
+        block_table, seq_lens, query_start = (t if t.dtype is i32 else t.to(i32) for t in (block_table, seq_lens, query_start))
+    if block_table.shape[1] > 1 and block_table.stride(1) != 1:
         block_table = block_table.contiguous()
     seq_lens, query_start = seq_lens.contiguous(), query_start.contiguous()
-    ks, vs = k_cache.stride(), v_cache.stride()
-    c = L.KvCache(k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), blocks, ks[0], ks[1], ks[2],
-                  vs[0], vs[1], vs[2], heads, size, dim, DT[k_cache.dtype])
-    b = L.KvBatch(block_table.data_ptr(), seq_lens.data_ptr(), query_start.data_ptr(), block_table.shape[1], block_table.stride(0),
-                  x.shape[0], batch, 0)
+    k0, k1, k2, _ = k_cache.stride()
+    v0, v1, v2, _ = v_cache.stride()
+    c = _KV_CACHE(k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), shape[0], k0, k1, k2, v0, v1, v2,
+                  shape[1], shape[2], shape[3], DT[dt])
+    b = _KV_BATCH(block_table.data_ptr(), seq_lens.data_ptr(), query_start.data_ptr(), block_table.shape[1], block_table.stride(0), x.shape[0], batch, 0)
     return c, b, (block_table, seq_lens, query_start)
+
+
+def _rows_of_heads(t, name, heads, dim):
+    """[tokens, heads, dim] with contiguous heads: as it is where it has them (a slice of a fused projection does), else a copy."""
+    shape = t.shape
+    if len(shape) != 3 or shape[1] != heads or shape[2] != dim:
+        raise ValueError(f"{name} must be [tokens, {heads}, {dim}], got {tuple(shape)}")
+    return t if t.stride(2) == 1 or dim == 1 else t.contiguous()
 
 
 def kv_cache_append(k, v, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, query_start) -> None:
@@ -709,20 +744,23 @@ def kv_cache_append(k, v, k_cache, v_cache, k_scale, v_scale, block_table, seq_l
 
     k_cache, v_cache [num_blocks, heads, block_size, head_dim] int8 or float8_e4m3fn (any strides, head_dim contiguous);
     k_scale, v_scale float32 [num_blocks, heads]; block_table [batch, width]; seq_lens [batch]: tokens of each request,
-    these rows included; query_start [batch + 1]: row offsets.  Row i of request b goes to position
+    these rows included; query_start [batch + 1]: row offsets, not decreasing.  Row i of request b goes to position
     seq_lens[b] - (query_start[b + 1] - query_start[b]) + i, slot position % block_size of block
     block_table[b, position // block_size].  The scale of a (block, head) is the symmetric min-max scale of the rows
     written to it; where the block already holds tokens of the request it never shrinks, and when it grows the older codes are
     rounded again.  Positions outside the table and blocks outside the cache are left out.  A block that is written must
     belong to one request."""
     if k_cache.dim() == 4:
-        k, v = (_rows_of_heads(t, n, k_cache.shape[1], k_cache.shape[3]) for t, n in ((k, "k"), (v, "v")))
+        _, heads, _, dim = k_cache.shape
+        k, v = _rows_of_heads(k, "k", heads, dim), _rows_of_heads(v, "v", heads, dim)
     if k.dtype is not v.dtype or k.shape != v.shape:
         raise ValueError(f"k and v must have one shape and dtype, got {tuple(k.shape)} {k.dtype} and {tuple(v.shape)} {v.dtype}")
     c, b, keep = _kv_structs(k, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, query_start)
-    _same_device(k, v)
-    _call(k.device, lib().ctb_kv_cache_append, ctypes.addressof(c), ctypes.addressof(b), k.data_ptr(), v.data_ptr(), DT[k.dtype],
-          k.stride(0), k.stride(1), v.stride(0), v.stride(1))
+    if v.get_device() != k.get_device():
+        _same_device(k, v)
+    k0, k1, _ = k.stride()
+    v0, v1, _ = v.stride()
+    _call(k.get_device(), lib().ctb_kv_cache_append, c, b, k.data_ptr(), v.data_ptr(), DT[k.dtype], k0, k1, v0, v1)
 
 
 def kv_cache_attention(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, query_start, softmax_scale=None, causal=True,
@@ -731,21 +769,25 @@ def kv_cache_attention(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_l
 
     q [tokens, q_heads, head_dim] bf16 / f16, q_heads a multiple of the cache's heads (query head h reads cache head
     h // (q_heads // heads)); rows query_start[b] .. query_start[b + 1] are the last tokens of request b, whose keys and
-    values are in the cache already.  softmax_scale defaults to head_dim ** -0.5.  With `causal` a query sees the positions
-    up to its own, otherwise all of its request.  Queries that see nothing give zeros.  return_lse: also the logarithm of the
-    softmax denominator, float32 [tokens, q_heads] (-inf for those queries)."""
+    values are in the cache already.  Scales are not negative.  softmax_scale defaults to head_dim ** -0.5.  With `causal` a query
+    sees the positions up to its own, otherwise all of its request.  Queries that see nothing give zeros.  return_lse: also the
+    logarithm of the softmax denominator, float32 [tokens, q_heads] (-inf for those queries)."""
     if k_cache.dim() == 4:
-        heads, dim = k_cache.shape[1], k_cache.shape[3]
-        if q.dim() != 3 or q.shape[2] != dim or q.shape[1] < 1 or q.shape[1] % max(heads, 1):
+        _, heads, _, dim = k_cache.shape
+        if q.dim() != 3 or q.shape[2] != dim or q.shape[1] < 1 or heads < 1 or q.shape[1] % heads:
             raise ValueError(f"q must be [tokens, a multiple of {heads}, {dim}], got {tuple(q.shape)}")
-        q = _rows_of_heads(q, "q", q.shape[1], dim)
+        if dim > 1 and q.stride(2) != 1:
+            q = q.contiguous()
     c, b, keep = _kv_structs(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, query_start)
-    tokens, q_heads, dim = q.shape
-    out = torch.empty((tokens, q_heads, dim), dtype=q.dtype, device=q.device)
-    lse = torch.empty((tokens, q_heads), dtype=torch.float32, device=q.device)
-    pc, pb = ctypes.addressof(c), ctypes.addressof(b)
-    nbytes = lib().ctb_kv_cache_attention_workspace_bytes(pc, pb, q_heads)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
-    _call(q.device, lib().ctb_kv_cache_attention, pc, pb, q.data_ptr(), DT[q.dtype], q.stride(0), q.stride(1), q_heads,
-          dim ** -0.5 if softmax_scale is None else float(softmax_scale), int(bool(causal)), out.data_ptr(), lse.data_ptr(), _dp(ws))
+    shape, device = q.shape, q.device
+    tokens, q_heads, dim = shape
+    out = torch.empty(shape, dtype=q.dtype, device=device)
+    lse = torch.empty(shape[:2], dtype=torch.float32, device=device)
+    library = lib()
+    nbytes = library.ctb_kv_cache_attention_workspace_bytes(c, b, q_heads)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+    q0, q1, _ = q.stride()
+    _call(device.index, library.ctb_kv_cache_attention, c, b, q.data_ptr(), DT[q.dtype], q0, q1, q_heads,
+          dim ** -0.5 if softmax_scale is None else float(softmax_scale), 1 if causal else 0, out.data_ptr(), lse.data_ptr(),
+          None if ws is None else ws.data_ptr())
     return (out, lse) if return_lse else out

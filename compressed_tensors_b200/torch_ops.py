@@ -418,6 +418,11 @@ def _no_grad_wanted(name, *tensors):
         raise RuntimeError(f"{name} computes no gradients: call it under torch.no_grad(), or use the dequantized weight")
 
 
+def _plain(t) -> bool:
+    """An ordinary tensor outside any tracing: the dispatcher has nothing to add to the call but its time."""
+    return type(t) in (Tensor, torch.nn.Parameter) and t.is_cuda and not torch.compiler.is_compiling() and torch._C._len_torch_dispatch_stack() == 0
+
+
 def _define(name: str, schema: str, fn, fake) -> None:
     _SERVING.define(f"{name}{schema}")
     _SERVING.impl(name, fn, "CompositeExplicitAutograd")
@@ -439,6 +444,9 @@ _define("dequantize_linear", "(Tensor x, Tensor q, Tensor scale, Tensor? zp, int
 
 def dequantize_linear(x, q, scale, zp=None, *, qtype, bits=4, col_group, scale_row_stride, codec="pack32", global_scale=None, bias=None):
     _no_grad_wanted("dequantize_linear", x, q, scale, global_scale, bias)
+    if _plain(x):
+        return _o.dequantize_linear(x, q, scale, zp, qtype=qtype, bits=bits, col_group=col_group, scale_row_stride=scale_row_stride,
+                                    codec=codec, global_scale=global_scale, bias=bias)
     return torch.ops.ctb200.dequantize_linear(x, q, scale, zp, qtype, bits, col_group, scale_row_stride, codec, global_scale, bias)
 
 
@@ -452,6 +460,8 @@ _define("kv_cache_append", "(Tensor k, Tensor v, Tensor(a!) k_cache, Tensor(b!) 
 
 def kv_cache_append(k, v, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, query_start) -> None:
     _no_grad_wanted("kv_cache_append", k, v)
+    if _plain(k):
+        return _o.kv_cache_append(k, v, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, query_start)
     torch.ops.ctb200.kv_cache_append(k, v, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, query_start)
 
 
@@ -472,6 +482,8 @@ _define("kv_cache_attention", "(Tensor q, Tensor k_cache, Tensor v_cache, Tensor
 def kv_cache_attention(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, query_start, softmax_scale=None, causal=True,
                        return_lse=False):
     _no_grad_wanted("kv_cache_attention", q)
+    if _plain(q):
+        return _o.kv_cache_attention(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, query_start, softmax_scale, causal, return_lse)
     out, lse = torch.ops.ctb200.kv_cache_attention(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, query_start,
                                                    softmax_scale, causal)
     return (out, lse) if return_lse else out
