@@ -176,8 +176,20 @@ __device__ __forceinline__ uint32_t code_word(uint32_t w) {
     return INT8 ? w ^ 0x80808080u : w;
 }
 
+// Rows in front of the first request and behind the last one: zeros.
+template <int DT, int D, int THREADS>
+__device__ __forceinline__ void att_idle_rows(const AttArgs &a) {
+    const int64_t lo = a.t.batch > 0 ? min(max((int64_t)a.t.query_start[0], (int64_t)0), a.t.tokens) : 0;
+    const int64_t hi = a.t.batch > 0 ? min(max((int64_t)a.t.query_start[a.t.batch], lo), a.t.tokens) : 0;
+    for (int64_t i = blockIdx.x; i < lo + a.t.tokens - hi; i += gridDim.x) {
+        const int64_t row = (i < lo ? i : hi + i - lo) * a.q_heads;
+        for (int j = threadIdx.x; j < a.q_heads * (D / 2); j += THREADS) store_half2<DT>((uint16_t *)a.out + row * D + 2 * j, 0.0f, 0.0f);
+        for (int j = threadIdx.x; j < a.q_heads; j += THREADS) a.lse[row + j] = -INFINITY;
+    }
+}
+
 // Blocks that an SM holds: what shared memory (head size 256) and registers (two row tiles at 128) leave room for.
-__host__ __device__ constexpr int att_blocks(int head_dim, int nt) { return head_dim == 256 || (head_dim == 128 && nt == 2) ? 2 : 3; }
+__host__ __device__ constexpr int att_blocks(int head_dim, int nt) { return nt == 16 ? 1 : head_dim == 256 || (head_dim == 128 && nt == 2) ? 2 : 3; }
 
 template <int DT, bool INT8, int D, int NT>
 __global__ void __launch_bounds__(kAttThreads, att_blocks(D, NT)) kv_attention_kernel(const __grid_constant__ AttArgs a) {
@@ -513,14 +525,260 @@ __global__ void __launch_bounds__(kAttThreads, att_blocks(D, NT)) kv_attention_k
         }
         if (threadIdx.x == 0 && !open && piece < a.slots) a.join[piece].last = 0;
     }
-    // rows in front of the first request and behind the last one: zeros
-    const int64_t lo = a.t.batch > 0 ? min(max((int64_t)a.t.query_start[0], (int64_t)0), a.t.tokens) : 0;
-    const int64_t hi = a.t.batch > 0 ? min(max((int64_t)a.t.query_start[a.t.batch], lo), a.t.tokens) : 0;
-    for (int64_t i = blockIdx.x; i < lo + a.t.tokens - hi; i += gridDim.x) {
-        const int64_t row = (i < lo ? i : hi + i - lo) * a.q_heads;
-        for (int j = threadIdx.x; j < a.q_heads * (D / 2); j += kAttThreads) store_half2<DT>((uint16_t *)a.out + row * D + 2 * j, 0.0f, 0.0f);
-        for (int j = threadIdx.x; j < a.q_heads; j += kAttThreads) a.lse[row + j] = -INFINITY;
+    att_idle_rows<DT, D, kAttThreads>(a);
+}
+
+// ---------------------------------------------------------------- many query rows per cache head (prompts)
+// A row tile is 128 query rows, 16 for each of eight warps; 64 cached tokens at a time are converted to f16 once for all of them in
+// shared memory and taken from there as the column operand of mma.m16n8k16 (S = Q K^T, O += P V, the weights staying in registers between
+// the two).  Number formats, scales and the lazily raised maximum are those of the kernel above, and so are the line of steps,
+// its pieces, and the second kernel that joins them.
+//
+// What bounds it: the matrix instructions (4 D operations per row and token); the codes are read and converted once per 128 rows.
+// While a tile is computed the codes of the next one are on their way in registers, its block numbers and scales one tile ahead of that.
+constexpr int kTileWarps = 8, kTileThreads = kTileWarps * 32, kTileTokens = 64;
+
+template <int DT, bool INT8, int D>
+__global__ void __launch_bounds__(kTileThreads, 1) kv_attention_tile_kernel(const __grid_constant__ AttArgs a) {
+    constexpr int NT = 16, ROWS = 128, KS = D / 16, PIECES = D / 16, PASS = kTileThreads / PIECES, LOADS = kTileTokens / PASS;
+    static_assert(LOADS * PASS == kTileTokens && PASS % 16 == 0, "rows that a pass of the block loads are whole steps");
+    constexpr int PITCH = D * 2;  // bytes of a converted row; its 16-byte pieces are permuted by the row's low bits
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ float4 s_meta[2][4];  // per step of the tile: key scale, log2 and inverse of the value scale, flags (1: there, 2: values count)
+    uint8_t *sk = smem, *sv = smem + kTileTokens * PITCH;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+    const KvSeq first = kv_lane_seq(a.t, a.capacity, 0);
+    grid_next();
+    const AttCut cut = att_cut<NT>(a, first);
+    if (blockIdx.x == 0 && threadIdx.x == 0) *a.pieces = (cut.total + cut.per - 1) / cut.per;
+    const int block_steps = a.c.block_size >> 4, copy_row = threadIdx.x / PIECES, copy_piece = threadIdx.x % PIECES;
+
+    for (uint32_t piece = blockIdx.x; (uint64_t)piece * cut.per < cut.total; piece += a.grid) {
+        const uint32_t p0 = piece * cut.per, p1 = min(cut.total, p0 + cut.per);
+        bool open = false;  // an item begins here and ends behind the piece
+        for (uint32_t pos = p0; pos < p1;) {
+            const AttItem it = att_find<NT>(a, cut, first, pos);
+            if (it.b < 0 || pos - it.begin >= it.span) break;  // (not with row offsets in order)
+            const KvSeq sq = it.s;
+            const int steps = (int)it.steps, s0 = (int)(pos - it.begin), s1 = min(steps, (int)(p1 - it.begin));
+            pos = min(p1, it.begin + it.span);
+            const int32_t *table = a.t.block_table + (int64_t)it.b * a.t.table_stride;
+            const int rows = sq.rows * a.group, row0 = it.tile * ROWS;
+            const int last_end = kv_end(sq, min(sq.rows - 1, (int)fastdiv((uint32_t)(row0 + ROWS - 1), a.by_group)), a.causal != 0);
+            const int first_end = kv_end(sq, fastdiv((uint32_t)row0, a.by_group), a.causal != 0);
+
+            // copies: this thread's piece of rows copy_row, + PASS, ... of a tile of four steps
+            uint4 kc[LOADS], vc[LOADS];
+            int page[LOADS];
+            float4 next_meta = make_float4(0, 0, 0, 0);
+            int meta_page = -1;
+            auto block_of = [&](int step) { return step < s1 ? __ldg(table + fastdiv((uint32_t)step, a.block_steps)) : -1; };
+            auto there = [&](int p) { return (uint32_t)p < (uint32_t)a.c.num_blocks; };
+            auto look_up = [&](int s) {  // of the tile that begins at step s
+#pragma unroll
+                for (int i = 0; i < LOADS; ++i) page[i] = block_of(s + (copy_row + i * PASS) / 16);
+                if (threadIdx.x < 4) meta_page = block_of(s + threadIdx.x);
+            };
+            auto load = [&](int s) {
+#pragma unroll
+                for (int i = 0; i < LOADS; ++i) {
+                    const int row = copy_row + i * PASS, step = s + row / 16;
+                    kc[i] = vc[i] = make_uint4(0, 0, 0, 0);
+                    if (there(page[i]) && s * 16 + row < last_end) {  // what no row sees reads as zeros
+                        const int slot = (int)((uint32_t)step - fastdiv((uint32_t)step, a.block_steps) * block_steps) * 16 + row % 16;
+                        kc[i] = __ldg((const uint4 *)((const uint8_t *)a.c.k + (int64_t)page[i] * a.c.k_block_stride + (int64_t)it.head * a.c.k_head_stride + slot * a.c.k_token_stride) + copy_piece);
+                        vc[i] = __ldg((const uint4 *)((const uint8_t *)a.c.v + (int64_t)page[i] * a.c.v_block_stride + (int64_t)it.head * a.c.v_head_stride + slot * a.c.v_token_stride) + copy_piece);
+                    }
+                }
+                if (threadIdx.x < 4) {
+                    const bool in = there(meta_page);
+                    next_meta.x = in ? __ldg(a.c.k_scale + (int64_t)meta_page * a.c.heads + it.head) : 0.0f;
+                    next_meta.y = in ? __ldg(a.c.v_scale + (int64_t)meta_page * a.c.heads + it.head) : 1.0f;
+                    next_meta.w = __int_as_float(in ? 1 : 0);
+                }
+            };
+            if (s0 < s1) {
+                look_up(s0);
+                load(s0);
+                look_up(s0 + 4);
+            }
+
+            // query rows 16 warp + g and + 8: row operand, elements 2t, 2t + 1 and 2t + 8, 2t + 9 of every 16
+            uint32_t qf[KS][4];
+            float f[2];   // score factors
+            int end[2];   // positions seen
+            const bool busy = row0 + warp * 16 < rows;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int r = row0 + warp * 16 + g + 8 * h, qi = (int)fastdiv((uint32_t)r, a.by_group);
+                const bool in = r < rows;
+                const uint32_t *qr = (const uint32_t *)((const uint16_t *)a.q + (int64_t)(sq.first_row + (in ? qi : 0)) * a.q_token_stride +
+                                                        (int64_t)(it.head * a.group + (in ? r - qi * a.group : 0)) * a.q_head_stride);
+                uint32_t most = 0;
+#pragma unroll
+                for (int k = 0; k < KS; ++k)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const uint32_t v = in ? __ldg(qr + k * 8 + t + 4 * j) : 0;
+                        qf[k][h + 2 * j] = v;
+                        most = max2_nan<DT>(most, v & 0x7fff7fffu);
+                    }
+                most = max2_nan<DT>(most, __shfl_xor_sync(0xffffffffu, most, 1));
+                most = max2_nan<DT>(most, __shfl_xor_sync(0xffffffffu, most, 2));
+                const float top = half_f32<DT>(max(most & 0xffffu, most >> 16));
+                const int e = max((int)(__float_as_uint(top) >> 23), 8);
+                const float up = __uint_as_float((uint32_t)(261 - e) << 23);  // the largest element comes to [128, 256)
+#pragma unroll
+                for (int k = 0; k < KS; ++k)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const uint32_t v = qf[k][h + 2 * j];
+                        qf[k][h + 2 * j] = pack_f16x2(half_f32<DT>(v & 0xffffu) * up, half_f32<DT>(v >> 16) * up);
+                    }
+                f[h] = a.scale_log2 * __uint_as_float((uint32_t)max(e - 7, 1) << 23);
+                end[h] = in ? kv_end(sq, qi, a.causal != 0) : 0;
+            }
+
+            float o[D / 8][4], m[2] = {-3.402823466e38f, -3.402823466e38f}, l[2] = {0.0f, 0.0f};
+#pragma unroll
+            for (int j = 0; j < D / 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.0f;
+
+            int buf = 0;
+            for (int s = s0; s < s1; s += 4, buf ^= 1) {
+                __syncthreads();  // the tile before has been read
+                // eight codes -> eight f16 in order
+                auto spread = [](uint32_t x, uint32_t y) {
+                    const uint32_t u = code_word<INT8>(x), v = code_word<INT8>(y);
+                    return make_uint4(code_pair<INT8, 0>(u), code_pair<INT8, 1>(u), code_pair<INT8, 0>(v), code_pair<INT8, 1>(v));
+                };
+#pragma unroll
+                for (int i = 0; i < LOADS; ++i) {
+                    const int row = copy_row + i * PASS, x = row & 7;
+                    uint8_t *kr = sk + row * PITCH, *vr = sv + row * PITCH;
+                    *(uint4 *)(kr + (((2 * copy_piece) ^ x) << 4)) = spread(kc[i].x, kc[i].y);
+                    *(uint4 *)(kr + (((2 * copy_piece + 1) ^ x) << 4)) = spread(kc[i].z, kc[i].w);
+                    *(uint4 *)(vr + (((2 * copy_piece) ^ x) << 4)) = spread(vc[i].x, vc[i].y);
+                    *(uint4 *)(vr + (((2 * copy_piece + 1) ^ x) << 4)) = spread(vc[i].z, vc[i].w);
+                }
+                if (threadIdx.x < 4) {
+                    const float vs = next_meta.y, vsafe = vs < 0x1p-120f ? 0x1p-120f : vs;  // as in the kernel above
+                    s_meta[buf][threadIdx.x] = make_float4(next_meta.x, log2f(vsafe), 1.0f / vsafe, __int_as_float(__float_as_int(next_meta.w) | (vs != 0.0f ? 2 : 0)));
+                }
+                if (s + 4 < s1) {
+                    load(s + 4);
+                    look_up(s + 8);
+                }
+                __syncthreads();
+                if (!busy) continue;
+                // scores of 16 rows x 64 tokens
+                float sc[8][4];
+#pragma unroll
+                for (int k = 0; k < KS; ++k)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {  // 16 tokens: two column tiles
+                        uint32_t b[4];
+                        const int row = j * 16 + (lane & 7) + ((lane >> 4) << 3);
+                        ldmatrix4(b, smem_u32(sk + row * PITCH + (((2 * k + ((lane >> 3) & 1)) ^ (row & 7)) << 4)));
+                        if (k == 0) {
+                            mma16816_first<CTB_F16>(sc[2 * j], qf[k][0], qf[k][1], qf[k][2], qf[k][3], b[0], b[1]);
+                            mma16816_first<CTB_F16>(sc[2 * j + 1], qf[k][0], qf[k][1], qf[k][2], qf[k][3], b[2], b[3]);
+                        } else {
+                            mma16816<CTB_F16>(sc[2 * j], qf[k][0], qf[k][1], qf[k][2], qf[k][3], b[0], b[1]);
+                            mma16816<CTB_F16>(sc[2 * j + 1], qf[k][0], qf[k][1], qf[k][2], qf[k][3], b[2], b[3]);
+                        }
+                    }
+                bool over = false;
+                float iv[4];
+                uint32_t keep[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float4 mt = s_meta[buf][j];
+                    const int flags = __float_as_int(mt.w), tok = (s + j) * 16;
+                    iv[j] = mt.z;
+                    keep[j] = flags & 2 ? 0xffffffffu : 0;
+                    const bool mask = !(flags & 1) || tok + 16 > first_end;
+#pragma unroll
+                    for (int c = 0; c < 2; ++c)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            float &x = sc[2 * j + c][i];
+                            x = fmaf(x, mt.x * f[i >> 1], mt.y);
+                            if (mask && (!(flags & 1) || tok + c * 8 + 2 * t + (i & 1) >= end[i >> 1])) x = -INFINITY;
+                            over |= x > m[i >> 1] + 8.0f;
+                        }
+                }
+                if (__any_sync(0xffffffffu, over)) {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        float x = -INFINITY;
+#pragma unroll
+                        for (int c = 0; c < 8; ++c) x = fmaxf(x, fmaxf(sc[c][2 * h], sc[c][2 * h + 1]));
+                        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
+                        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+                        const float mn = fmaxf(m[h], x), down = ex2(m[h] - mn);
+                        m[h] = mn;
+                        l[h] *= down;
+#pragma unroll
+                        for (int j = 0; j < D / 8; ++j) {
+                            o[j][2 * h] *= down;
+                            o[j][2 * h + 1] *= down;
+                        }
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {  // 16 tokens of weights: the row operand of the second product
+                    uint32_t p[4];
+#pragma unroll
+                    for (int c = 0; c < 2; ++c)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const float x = ex2(sc[2 * j + c][2 * h] - m[h]), y = ex2(sc[2 * j + c][2 * h + 1] - m[h]);
+                            l[h] = fmaf(x + y, iv[j], l[h]);
+                            p[2 * c + h] = pack_f16x2(x, y) & keep[j];
+                        }
+#pragma unroll
+                    for (int d = 0; d < D / 16; ++d) {
+                        uint32_t b[4];
+                        const int row = j * 16 + (lane & 15);
+                        ldmatrix4_trans(b, smem_u32(sv + row * PITCH + (((2 * d + (lane >> 4)) ^ (row & 7)) << 4)));
+                        mma16816<CTB_F16>(o[2 * d], p[0], p[1], p[2], p[3], b[0], b[1]);
+                        mma16816<CTB_F16>(o[2 * d + 1], p[0], p[1], p[2], p[3], b[2], b[3]);
+                    }
+                }
+            }
+
+            const bool whole = s0 == 0 && s1 == steps;
+            const int64_t slot = cut.padded ? piece : 2 * (int64_t)piece + (p0 < it.begin ? 1 : 0);
+            float *part = a.part + slot * ROWS * (D + 2);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+                l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+                const int r = warp * 16 + g + 8 * h, qi = (int)fastdiv((uint32_t)(row0 + r), a.by_group);
+                if (row0 + r >= rows) continue;
+                if (whole) {
+                    const int64_t row = (int64_t)(sq.first_row + qi) * a.q_heads + it.head * a.group + row0 + r - qi * a.group;
+                    const float inv = l[h] == 0.0f ? 0.0f : 1.0f / l[h];  // nothing seen: zeros
+#pragma unroll
+                    for (int j = 0; j < D / 8; ++j) store_half2<DT>((uint16_t *)a.out + row * D + j * 8 + 2 * t, o[j][2 * h] * inv, o[j][2 * h + 1] * inv);
+                    if (t == 0) a.lse[row] = l[h] == 0.0f ? -INFINITY : (m[h] + log2f(l[h])) * 0.6931471805599453f;
+                } else if (slot < a.slots) {
+                    float *pr = part + r * (D + 2);
+#pragma unroll
+                    for (int j = 0; j < D / 8; ++j) *(float2 *)(pr + j * 8 + 2 * t) = make_float2(o[j][2 * h], o[j][2 * h + 1]);
+                    if (t == 0) *(float2 *)(pr + D) = make_float2(m[h], l[h]);
+                }
+            }
+            if (threadIdx.x == 0 && s1 < steps && it.begin >= p0 && piece < a.slots) {
+                const int qi = (int)fastdiv((uint32_t)row0, a.by_group);
+                a.join[piece] = AttJoin{(int64_t)(sq.first_row + qi) * a.q_heads + it.head * a.group, slot, (it.begin + (uint32_t)steps - 1) / cut.per,
+                                        min(ROWS, rows - row0), row0 - qi * a.group, cut.padded};
+                open = true;
+            }
+        }
+        if (threadIdx.x == 0 && !open && piece < a.slots) a.join[piece].last = 0;
     }
+    att_idle_rows<DT, D, kTileThreads>(a);
 }
 
 // Joins what the pieces of an item left in scratch: block c takes the item that begins in piece c and ends behind it.
@@ -539,7 +797,8 @@ __global__ void __launch_bounds__(kJoinWarps * 32) kv_attention_join_kernel(cons
         const uint32_t c = c0 + (__ffs(todo) - 1) * gridDim.x;
         const AttJoin it = a.join[c];
         const uint32_t last = it.last;
-        const int n = it.rows;
+        const int base = blockIdx.y * kJoinWarps, n = min(it.rows - base, kJoinWarps);  // rows base .. base + n of the tile
+        if (n <= 0) continue;
         // all warps on the rows: 16 / (n rounded up to a power of two) of them on each, every one with its share of the pieces
         const int log_rows = n <= 1 ? 0 : 32 - __clz(n - 1), log_warps = 4 - log_rows, r = warp & ((1 << log_rows) - 1);
         float top = -3.402823466e38f, sum = 0.0f, v[E];
@@ -557,7 +816,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) kv_attention_join_kernel(cons
                     for (int e = 0; e < E; ++e) x[i][e] = 0.0f;
                     const int64_t slot = p == c ? it.slot : it.padded ? p : 2 * (int64_t)p;
                     if (p <= last && slot < a.slots) {
-                        const float *part = a.part + (slot * ROWS + r) * (D + 2);
+                        const float *part = a.part + (slot * ROWS + base + r) * (D + 2);
                         ml[i] = __ldcg((const float2 *)(part + D));
 #pragma unroll
                         for (int e = 0; e < E; e += 2) *(float2 *)&x[i][e] = __ldcg((const float2 *)(part + lane * E + e));
@@ -595,7 +854,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) kv_attention_join_kernel(cons
                 x0 = fmaf(s_v[k][d], down, x0);
                 x1 = fmaf(s_v[k][d + 1], down, x1);
             }
-            const int rr = it.first + q, qi = (int)fastdiv((uint32_t)rr, a.by_group);
+            const int rr = it.first + base + q, qi = (int)fastdiv((uint32_t)rr, a.by_group);
             const int64_t row = it.row + (int64_t)qi * a.q_heads + rr - qi * a.group;
             const float inv = total == 0.0f ? 0.0f : 1.0f / total;
             store_half2<DT>((uint16_t *)a.out + row * D + d, x0 * inv, x1 * inv);
@@ -611,9 +870,12 @@ static int64_t att_items(const ctb_kv_cache &c, const ctb_kv_batch &t, int group
     return (int64_t)c.heads * ((t.tokens * group + rows - 1) / rows + t.batch);  // a tile for every `rows` query rows, and one more per request
 }
 
+// Row tiles of a call, in eights: 128 rows on average from 48 rows per request on, where the conversions that the tile kernel saves
+// outweigh the rows that it computes for nothing; two eights from nine rows on; head size 256 has registers for one eight only.
 static int att_nt(const ctb_kv_cache &c, const ctb_kv_batch &t, int group) {
-    // two tiles of eight rows per step where a request has more than eight rows on average; head size 256 has registers for one
-    return c.head_dim <= 128 && t.tokens * group > 8 * (int64_t)t.batch ? 2 : 1;
+    const int64_t rows = t.tokens * group;
+    if (c.head_dim == 256) return 1;
+    return rows > 48 * (int64_t)t.batch ? 16 : rows > 8 * (int64_t)t.batch ? 2 : 1;
 }
 
 static int att_grid(int head_dim, int nt) { return sm_count() * att_blocks(head_dim, nt); }
@@ -636,6 +898,14 @@ int64_t kv_attention_workspace(const ctb_kv_cache &c, const ctb_kv_batch &t, int
     return 32 + att_slots(c, t, group, nt) * ((int64_t)sizeof(AttJoin) + 8 * nt * (c.head_dim + 2) * 4);
 }
 
+template <int DT, int D, int NT>
+static int att_finish(const AttArgs &a, cudaStream_t st) {
+    // no request is longer than the shortest piece, and there is a block for each: nothing to join
+    if (a.capacity <= kAttMinPiece * 16 && att_items(a.c, a.t, a.group, NT * 8) <= a.grid) return CTB_OK;
+    return launch_dependent("kv_attention_join_kernel", kv_attention_join_kernel<DT, D, NT>, dim3((unsigned)sm_count(), (NT * 8 + kJoinWarps - 1) / kJoinWarps),
+                            kJoinWarps * 32, 0, st, a);
+}
+
 template <int DT, bool INT8, int D, int NT>
 static int att_launch(const AttArgs &a, cudaStream_t st) {
     auto kernel = kv_attention_kernel<DT, INT8, D, NT>;
@@ -646,9 +916,19 @@ static int att_launch(const AttArgs &a, cudaStream_t st) {
     if (rc) return rc;
     kernel<<<a.grid, kAttThreads, bytes, st>>>(a);
     rc = after_launch("kv_attention_kernel");
-    // no request is longer than the shortest piece, and there is a block for each: nothing to join
-    if (rc || (a.capacity <= kAttMinPiece * 16 && att_items(a.c, a.t, a.group, NT * 8) <= a.grid)) return rc;
-    return launch_dependent("kv_attention_join_kernel", kv_attention_join_kernel<DT, D, NT>, dim3((unsigned)sm_count()), kJoinWarps * 32, 0, st, a);
+    return rc ? rc : att_finish<DT, D, NT>(a, st);
+}
+
+template <int DT, bool INT8, int D>
+static int att_tile_launch(const AttArgs &a, cudaStream_t st) {
+    auto kernel = kv_attention_tile_kernel<DT, INT8, D>;
+    constexpr size_t bytes = (size_t)2 * kTileTokens * D * 2;
+    static std::atomic<bool> ready[64];
+    int rc = allow_smem(kernel, bytes, ready);
+    if (rc) return rc;
+    kernel<<<a.grid, kTileThreads, bytes, st>>>(a);
+    rc = after_launch("kv_attention_tile_kernel");
+    return rc ? rc : att_finish<DT, D, 16>(a, st);
 }
 
 int kv_attention_launch(const ctb_kv_cache &c, const ctb_kv_batch &t, const void *q, int dtype, int64_t q_token_stride, int64_t q_head_stride, int q_heads,
@@ -678,6 +958,7 @@ int kv_attention_launch(const ctb_kv_cache &c, const ctb_kv_batch &t, const void
     auto go = [&](auto dt, auto i8) {
         constexpr int DT = decltype(dt)::value;
         constexpr bool I8 = decltype(i8)::value;
+        if (nt == 16) return c.head_dim == 64 ? att_tile_launch<DT, I8, 64>(a, st) : att_tile_launch<DT, I8, 128>(a, st);
         if (c.head_dim == 64) return nt == 1 ? att_launch<DT, I8, 64, 1>(a, st) : att_launch<DT, I8, 64, 2>(a, st);
         if (c.head_dim == 128) return nt == 1 ? att_launch<DT, I8, 128, 1>(a, st) : att_launch<DT, I8, 128, 2>(a, st);
         return att_launch<DT, I8, 256, 1>(a, st);
