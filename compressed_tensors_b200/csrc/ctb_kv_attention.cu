@@ -76,11 +76,12 @@ __device__ __forceinline__ uint32_t att_steps(const AttArgs &a, const KvSeq &s, 
     const int last = min(s.rows - 1, (int)fastdiv((uint32_t)((tile + 1) * NT * 8 - 1), a.by_group));
     return (uint32_t)(kv_end(s, last, a.causal != 0) + 15) >> 4;
 }
-// places that an item takes on the line; one without a step has its place too, and is written there
+// Places that an item takes on the line: its steps, and some for what every item costs besides (rows, first copies, results: about as
+// long as kAttItemSteps steps); an item without a step has its place too, and is written there.  On a padded line: whole pieces.
+constexpr uint32_t kAttItemSteps = 8;
 __device__ __forceinline__ uint32_t att_span(const AttCut &cut, uint32_t n) {
     static_assert(kAttMinPiece == 16, "pieces of a padded line");
-    n = max(n, 1u);
-    return cut.padded ? (n + 15) & ~15u : n;
+    return cut.padded ? (max(n, 1u) + 15) & ~15u : n + kAttItemSteps;
 }
 
 // steps of all tiles of a request, for one head
@@ -129,7 +130,7 @@ struct AttItem {
 // The item that holds position `pos` of the line.
 template <int NT>
 __device__ __forceinline__ AttItem att_find(const AttArgs &a, const AttCut &cut, const KvSeq &first, uint32_t pos) {
-    AttItem it;
+    AttItem it = {};
     const uint32_t heads = (uint32_t)a.c.heads;
     it.b = kv_locate(a.t, a.capacity, first, pos, [&](const KvSeq &q) { return att_request_steps<NT>(a, q, cut) * heads; }, it.s, it.begin);
     const int tiles = it.b < 0 ? 0 : att_tiles<NT>(a, it.s);
@@ -142,6 +143,20 @@ __device__ __forceinline__ AttItem att_find(const AttArgs &a, const AttCut &cut,
     it.head = heads == 1 || it.span == 0 ? 0 : (int)((pos - it.begin) / it.span);
     it.begin += it.head * it.span;
     return it;
+}
+
+// The item behind `it` on the line.
+template <int NT>
+__device__ __forceinline__ void att_next(const AttArgs &a, const AttCut &cut, const KvSeq &first, AttItem &it) {
+    it.begin += it.span;
+    if (++it.head < a.c.heads) return;
+    it.head = 0;
+    if (++it.tile < att_tiles<NT>(a, it.s)) {
+        it.steps = att_steps<NT>(a, it.s, it.tile);
+        it.span = att_span(cut, it.steps);
+    } else {
+        it = att_find<NT>(a, cut, first, it.begin);
+    }
 }
 
 // A step in shared memory: 16 key rows, then 16 value rows.  Rows are copied whole and in order, 16 bytes per lane (with a
@@ -211,12 +226,13 @@ __global__ void __launch_bounds__(kAttThreads, att_blocks(D, NT)) kv_attention_k
     for (uint32_t piece = blockIdx.x; (uint64_t)piece * cut.per < cut.total; piece += a.grid) {
         const uint32_t p0 = piece * cut.per, p1 = min(cut.total, p0 + cut.per);
         bool open = false;  // an item begins here and ends behind the piece
-        for (uint32_t pos = p0; pos < p1;) {
-            const AttItem it = att_find<NT>(a, cut, first, pos);
+        AttItem it = att_find<NT>(a, cut, first, p0);
+        for (uint32_t pos = p0; pos < p1; att_next<NT>(a, cut, first, it)) {
             if (it.b < 0 || pos - it.begin >= it.span) break;  // (not with row offsets in order)
             const KvSeq sq = it.s;
             const int steps = (int)it.steps, s0 = (int)(pos - it.begin), s1 = min(steps, (int)(p1 - it.begin));
             pos = min(p1, it.begin + it.span);
+            if (s0 > 0 && s0 >= steps) continue;  // nothing but the end of its place is in this piece
             // this warp's steps: s0 + warp, + 4, ...; what has to be known of 32 of them at a time, one per lane
             const int mine = s1 - s0 > warp ? (s1 - s0 - warp + kAttWarps - 1) / kAttWarps : 0;
             const int32_t *table = a.t.block_table + (int64_t)it.b * a.t.table_stride;
@@ -556,12 +572,13 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attention_tile_kernel(cons
     for (uint32_t piece = blockIdx.x; (uint64_t)piece * cut.per < cut.total; piece += a.grid) {
         const uint32_t p0 = piece * cut.per, p1 = min(cut.total, p0 + cut.per);
         bool open = false;  // an item begins here and ends behind the piece
-        for (uint32_t pos = p0; pos < p1;) {
-            const AttItem it = att_find<NT>(a, cut, first, pos);
+        AttItem it = att_find<NT>(a, cut, first, p0);
+        for (uint32_t pos = p0; pos < p1; att_next<NT>(a, cut, first, it)) {
             if (it.b < 0 || pos - it.begin >= it.span) break;  // (not with row offsets in order)
             const KvSeq sq = it.s;
             const int steps = (int)it.steps, s0 = (int)(pos - it.begin), s1 = min(steps, (int)(p1 - it.begin));
             pos = min(p1, it.begin + it.span);
+            if (s0 > 0 && s0 >= steps) continue;  // nothing but the end of its place is in this piece
             const int32_t *table = a.t.block_table + (int64_t)it.b * a.t.table_stride;
             const int rows = sq.rows * a.group, row0 = it.tile * ROWS;
             const int last_end = kv_end(sq, min(sq.rows - 1, (int)fastdiv((uint32_t)(row0 + ROWS - 1), a.by_group)), a.causal != 0);
@@ -900,8 +917,8 @@ int64_t kv_attention_workspace(const ctb_kv_cache &c, const ctb_kv_batch &t, int
 
 template <int DT, int D, int NT>
 static int att_finish(const AttArgs &a, cudaStream_t st) {
-    // no request is longer than the shortest piece, and there is a block for each: nothing to join
-    if (a.capacity <= kAttMinPiece * 16 && att_items(a.c, a.t, a.group, NT * 8) <= a.grid) return CTB_OK;
+    // no request is longer than the shortest piece, and so few that the line is a padded one: nothing to join
+    if (a.capacity <= kAttMinPiece * 16 && att_items(a.c, a.t, a.group, NT * 8) * (kAttMinPiece + (int)kAttItemSteps) <= (int64_t)kAttMinPiece * a.grid) return CTB_OK;
     return launch_dependent("kv_attention_join_kernel", kv_attention_join_kernel<DT, D, NT>, dim3((unsigned)sm_count(), (NT * 8 + kJoinWarps - 1) / kJoinWarps),
                             kJoinWarps * 32, 0, st, a);
 }

@@ -45,6 +45,8 @@ __device__ __forceinline__ int kv_locate(const ctb_kv_batch &t, int64_t capacity
         }
         run = __shfl_sync(0xffffffffu, upto, 31);
     }
+    s = KvSeq{0, 0, 0, 0};
+    begin = run;
     return -1;
 }
 
