@@ -433,6 +433,53 @@ def decode_step(state):
     return y, att, lse, call_linear(o, x=att.flatten(1))
 
 
+@pytest.mark.parametrize("fmt, kw", [("pack-quantized", dict(num_bits=4, symmetric=True, strategy="group", group_size=128)),
+                                     ("pack-quantized", dict(num_bits=4, symmetric=False, strategy="group", group_size=32)),
+                                     ("pack-quantized", dict(num_bits=4, symmetric=True, strategy="channel")),
+                                     ("nvfp4-pack-quantized", dict(num_bits=4, type="float", symmetric=True, strategy="tensor_group", group_size=16))])
+def test_compressed_linear_keeps_its_packed_weight(fmt, kw):
+    from compressed_tensors_b200 import _lib as L
+    from compressed_tensors_b200.compressors import ModelCompressor
+    from compressed_tensors_b200.linear import CompressedLinear
+    from compressed_tensors_b200.quantization import (QuantizationArgs, QuantizationConfig, QuantizationScheme, QuantizationStatus, apply_quantization_config,
+                                                      calibrate_weight_qparams)
+
+    torch.manual_seed(3)
+    model = torch.nn.Sequential(torch.nn.Linear(384, 200, bias=True)).to(torch.bfloat16).cuda()
+    scheme = QuantizationScheme(targets=["Linear"], weights=QuantizationArgs(**kw))
+    cfg = QuantizationConfig(config_groups={"g": scheme}, format=fmt)
+    apply_quantization_config(model, cfg)
+    calibrate_weight_qparams(model[0])
+    bias = model[0].bias.data.clone()
+    sd = ModelCompressor(quantization_config=cfg).compress(model)
+    mods = []
+    for keep in (True, False):
+        lin = torch.nn.Linear(384, 200, bias=True, dtype=torch.bfloat16).cuda()
+        mod = CompressedLinear.from_linear(lin, scheme, fmt, keep_packed=keep)
+        _, unexpected = mod.load_state_dict({k.removeprefix("0."): v for k, v in sd.items() if k.startswith("0.")}, strict=False)
+        assert not unexpected
+        mods.append(mod)
+    packed, dense = mods
+    weight = dense.compressor.decompress_module(dense).double()
+    with torch.no_grad():
+        for tokens in (1, 7, 32):
+            x = torch.randn(tokens, 384, dtype=torch.bfloat16, device="cuda")
+            assert packed.packed_product(x) is not None
+            y = packed(x)
+            want, size = x.double() @ weight.t() + bias.double(), x.double().abs() @ weight.abs().t() + bias.double().abs()
+            # the dense weight is rounded to bf16 (half a step each), the packed product does not round it
+            assert bool(((y.double() - want).abs() <= 2.0 ** -8 * want.abs() + (2.0 ** -8 + 96 * 2.0 ** -23) * size).all())
+            assert packed.quantization_status == QuantizationStatus.COMPRESSED and not hasattr(packed, "weight")
+        many = torch.randn(33, 384, dtype=torch.bfloat16, device="cuda")
+        assert packed.packed_product(many) is None and packed.packed_product(many[:2].float()) is None
+        assert torch.equal(packed(many), dense(many))
+    few = torch.randn(3, 384, dtype=torch.bfloat16, device="cuda", requires_grad=True)
+    assert packed.packed_product(few) is None  # a gradient is wanted: the dense way gives it
+    packed(few).sum().backward()
+    assert bool(((few.grad[0].double() - weight.sum(0)).abs() <= 2.0 ** -8 * weight.sum(0).abs() + 200 * 2.0 ** -23 * weight.abs().sum(0)).all())
+    assert L.launch_count() > 0
+
+
 def test_a_decoding_step():
     state = decode_state()
     c, qkv, o, x, qs, (q_heads, heads, dim) = state
