@@ -21,8 +21,8 @@ __all__ = ["CompressedLinear"]
 
 class CompressedLinear(Linear):
     keep_packed = False
-    # From here on a decompression and one library product take less than the packed product, which reads the weight once for every 32
-    # tokens (14336 x 4096: 51 us for 32 tokens, 100 for 64; dequantize and product about 60).
+    # Above this a decompression and one library product take less than the packed product, which reads the weight again for every 32
+    # tokens (14336 x 4096: 19 us for 16 tokens, 36 for 32, twice that for 33, against 43 to 44 for dequantize and product).
     packed_tokens = 32
 
     def __init__(self, *args, **kwargs) -> None:

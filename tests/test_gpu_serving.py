@@ -73,7 +73,7 @@ def check_linear(s, got, x=None):
                                               ("pack32", -1, True), ("fp4x2", 16, False), ("fp4x2", 32, False)])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("tokens, rows, cols", [(1, 128, 128), (1, 1000, 2048), (3, 17, 4096), (8, 129, 1664), (9, 256, 384), (16, 1, 256), (31, 200, 640), (33, 144, 256),
-                                                (70, 96, 512)])
+                                                (70, 96, 512), (10, 8200, 256), (24, 8192, 512)])
 def test_linear(tokens, rows, cols, codec, group, zp, dtype):
     s = make_linear(tokens, rows, cols, codec, group, zp, tokens % 2 == 1, dtype, torch.float8_e4m3fn if codec == "fp4x2" else dtype, seed=tokens)
     check_linear(s, call_linear(s))
