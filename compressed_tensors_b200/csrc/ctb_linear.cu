@@ -1,7 +1,8 @@
 // Product with a 4-bit weight: out[t][n] = sum_k x[t][k] * (code[n][k] - zp) * scale (+ bias[n]), for few tokens.
 //
 // What bounds it: a weight code is used once per token, so at a few tokens the call takes the time of reading the
-// packed weight (half a byte per weight) from HBM.
+// packed weight (half a byte per weight) from HBM.  128256 x 4096 by one token: 60 us, 4.5 TB/s of weight; 14336 x 4096: 13 us by one
+// token, 15 by 8, 19 by 16, 36 by 32; below about 30 MB the ramp and the instructions (about 170 per 2048 weights and warp) show.
 #include <atomic>
 
 #include "ctb_fastdiv.h"

@@ -525,6 +525,42 @@ def test_captured_steps_share_nothing():
                 s[0]["seq_lens"] += 1
 
 
+@pytest.mark.parametrize("rows", [1, 40])
+def test_a_captured_attention_follows_its_lengths(rows):
+    """Requests long enough to be cut into pieces that a second kernel joins; lengths and queries change between replays."""
+    c = make_cache([6000, 700, 40], 2, 128, 64, torch.float8_e4m3fn)
+    c["seq_lens"] = torch.tensor([100, 60, 40], dtype=torch.int32, device="cuda")
+    qs, tokens = starts([rows] * 3, extra=1)
+    q = torch.randn(tokens, 8, 128, generator=gen(1), device="cuda").to(torch.bfloat16)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call_attention(c, q, qs)
+    torch.cuda.current_stream().wait_stream(side)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = call_attention(c, q, qs)
+    for i, lens in enumerate(([100, 60, 40], [6000, 700, 40], [0, 1, 0], [5990, 0, 33])):
+        c["seq_lens"].copy_(torch.tensor(lens, dtype=torch.int32))
+        q.copy_(torch.randn(tokens, 8, 128, generator=gen(i), device="cuda").to(torch.bfloat16))
+        g.replay()
+        check_attention(c, q, qs, *out)
+        eager = call_attention(c, q, qs)
+        assert torch.equal(eager[0], out[0]) and torch.equal(eager[1], out[1])
+
+
+def test_many_requests():
+    """More requests than a warp has lanes, with empty ones between."""
+    lens = [(37 * i) % 301 for i in range(150)]
+    rows = [0 if i % 7 == 3 else 1 + (i % 3 == 0) for i in range(150)]
+    lens = [max(n, r) if i % 5 else n for i, (n, r) in enumerate(zip(lens, rows))]
+    c = make_cache(lens, 2, 64, 16, torch.int8)
+    qs, tokens = starts(rows, extra=3)
+    fused = torch.randn(tokens, 12, 64, generator=gen(4), device="cuda").to(torch.float16)
+    check_append(c, fused[:, 8:10], fused[:, 10:], qs)
+    check_attention(c, fused[:, :8], qs, *call_attention(c, fused[:, :8], qs))
+
+
 def test_calls_on_two_streams_at_once():
     states = [decode_state(s) for s in (3, 4)]
     want = [decode_step(decode_state(s)) for s in (3, 4)]
